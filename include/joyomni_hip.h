@@ -496,6 +496,110 @@ int jo_kv_commit_rope(const void* src_k, const void* src_v, void* dst_k, void* d
                       int64_t table_stride, int64_t table_batch_stride, int dtype,
                       void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving over a paged KV pool: many streams' keys and values in pages of one
+ * pool, [num_pages, page_size, kv_heads, head_dim], and a block table [requests,
+ * width] that lists each request's pages in order. A reference process serves
+ * one stream from a contiguous pool (deploy/xvideo/serving/graph_runner.py:49-60,
+ * 137-142); these entry points have no counterpart there.
+ *
+ * Lengths, tables and slots are int32 / int64 DEVICE arrays, so a step's calls
+ * need nothing from the host but its fixed sizes and can be captured once and
+ * replayed. What they hold is checked where it is used: a page id outside
+ * [0, num_pages) names no page, a slot outside the pool no place, and no value
+ * makes a kernel read or write outside the arrays' stated sizes.
+ *
+ * These entry points came after version 5's others; no argument list changed,
+ * so the version stays.
+ * ------------------------------------------------------------------------ */
+
+/* Tables of a step from request lengths. ctx_lens[r]: tokens already cached,
+ * new_lens[r]: tokens of this step (negative counts as 0), free_pages: a stack
+ * of page ids whose first *num_free entries are free. With P = page_size and
+ * W = table_width:
+ *   cu_q[0] = 0, cu_q[r+1] = min(cu_q[r] + new_lens[r], max_tokens)
+ *   kv_lens[r] = ctx_lens[r] + cu_q[r+1] - cu_q[r]
+ *   block_table[r, j] for ceil(ctx_lens[r] / P) <= j < min(W, ceil(kv_lens[r] / P)):
+ *     pages from the top of the stack, request after request; -1 where the
+ *     stack has run out or holds no page id (other entries stay as they are)
+ *   slots[t] = page * P + place of token t's position in its request; -1 for a
+ *     token without a page and for t >= cu_q[requests]
+ *   *free_left = *num_free - pages taken (negative: so many are missing)
+ * *num_free counts as at most free_capacity. The stack itself is only read: the
+ * next step's *num_free is *free_left when pages were not missing. Sizes of
+ * outputs: cu_q requests + 1, kv_lens requests, slots max_tokens. requests <=
+ * 4096. */
+int jo_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens, int64_t requests,
+                    int32_t* block_table, int64_t table_stride, int64_t table_width,
+                    const int32_t* free_pages, int64_t free_capacity, const int32_t* num_free,
+                    int64_t page_size, int64_t num_pages, int64_t max_tokens, int32_t* cu_q,
+                    int32_t* kv_lens, int64_t* slots, int32_t* free_left, void* stream);
+
+/* jo_kv_commit_rope with the rows sent to pages:
+ *   pages_k[l, slots[n] / P, slots[n] % P, :] = apply_rotary_emb(src_k[l, n, :], cos[n], sin[n])
+ *   pages_v[l, slots[n] / P, slots[n] % P, :] = src_v[l, n, :]      (when src_v != NULL)
+ * with the same rounding, bit for bit; K is copied as it is when cos and sin
+ * are NULL. A row whose slot lies outside [0, num_pages * page_size) is left
+ * out. Slots of one call must differ (of two rows sent to one place parts of
+ * either may remain). src: [layers, tokens, num_heads * head_dim]; pages:
+ * [layers, num_pages, page_size, num_heads * head_dim], element strides, token
+ * rows contiguous; fewer than 2^32 tokens in a pool. */
+int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, void* pages_k, void* pages_v,
+                            int64_t layers, int64_t tokens, int64_t num_heads, int64_t head_dim,
+                            int64_t src_layer_stride, int64_t src_token_stride,
+                            int64_t pages_layer_stride, int64_t page_stride,
+                            int64_t pages_token_stride, int64_t num_pages, int64_t page_size,
+                            const int64_t* slots, const float* cos, const float* sin,
+                            int64_t table_stride, int dtype, void* stream);
+
+/* Attention of packed query tokens over keys and values of their own request.
+ * Request r has the query tokens cu_q[r] .. cu_q[r+1]-1 (n_r of them) and m_r
+ * keys; query head h reads key head h / (q_heads / kv_heads):
+ *   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j]   over the keys j that i sees:
+ *     j < m_r, and with causal != 0 also j <= m_r - n_r + (i's place in its request)
+ * A token that sees no key gets zeros. Scores, maxima, sums and the output's
+ * accumulation are fp32; the probabilities are rounded to dtype before they
+ * meet v. A key that a token does not see has no part in its result, NaN and
+ * infinities included. Tokens that belong to no request (behind cu_q[requests])
+ * get zeros when fill_rest != 0 and keep what they hold otherwise.
+ *   _varlen: k, v [kv_tokens, kv_heads, head_dim] packed as q is, request r's
+ *     at cu_k[r] .. cu_k[r+1]-1 (cu_k = cu_q for self-attention of prompts).
+ *   _paged: key j of request r at place j % page_size of page
+ *     block_table[r, j / page_size]; m_r = kv_lens[r], of which the first
+ *     table_width * page_size have a place. Keys of an entry that names no page
+ *     are not seen.
+ * q, out: [q_tokens, q_heads, head_dim]. All strides in elements, multiples of
+ * 8, tensors 16-byte aligned, head_dim contiguous: 64, 128 or 256. dtype bf16 or
+ * fp16, q_heads a multiple of kv_heads, scale > 0. out overlaps no input.
+ * cu_q, cu_k: int32 [requests + 1], non-decreasing from 0 on.
+ * The workspace (jo_attention_workspace_bytes, 16-byte aligned; NULL with 0
+ * bytes: keys are not split) holds partial results of split key ranges; it is
+ * in use until the work queued on `stream` finishes. */
+int jo_attention_varlen(const void* q, const void* k, const void* v, void* out, int64_t q_tokens,
+                        int64_t kv_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                        int64_t v_head_stride, int64_t out_token_stride, int64_t out_head_stride,
+                        const int32_t* cu_q, const int32_t* cu_k, float scale, int causal,
+                        int fill_rest, int dtype, void* workspace, int64_t workspace_bytes,
+                        void* stream);
+int jo_attention_paged(const void* q, const void* pages_k, const void* pages_v, void* out,
+                       int64_t q_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                       int64_t head_dim, int64_t num_pages, int64_t page_size,
+                       int64_t q_token_stride, int64_t q_head_stride, int64_t k_page_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_page_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int64_t out_token_stride,
+                       int64_t out_head_stride, const int32_t* block_table, int64_t table_stride,
+                       int64_t table_width, const int32_t* cu_q, const int32_t* kv_lens,
+                       float scale, int causal, int fill_rest, int dtype, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes that the two calls above use for these sizes (0: none);
+ * kv_capacity is kv_tokens, or table_width * page_size. A host-side
+ * computation. */
+int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests, int64_t q_heads,
+                                     int64_t kv_heads, int64_t head_dim, int64_t kv_capacity);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -18,6 +18,11 @@
 // waves of their own, after all the K waves. A lane's table columns repeat
 // every head (512 elements per pass is a whole number of heads when D divides
 // 512), so a lane reads its 8 cos and 8 sin values once per row.
+//
+// The paged form sends row n of every layer to the page and place that slots[n]
+// names (slot = page * page_size + place) instead of to token d_off + n, and
+// leaves out rows whose slot lies outside the pool. Without tables K is copied
+// as V is. The slot is loaded beside the row, not before it.
 
 #include <type_traits>
 
@@ -42,7 +47,20 @@ struct CommitArgs {
   const float* sin;          // (tab_bs 0: one table for every batch row)
   int64_t tab_ts, tab_bs;
   FastDiv fd_tokens, fd_batch;  // the row index's divisors (set by launch_commit)
+  // Paged destination: token row of page p at l * d_ls + p * d_ps + place * d_ts.
+  const int64_t* slots;
+  int64_t n_slots;  // pages * page_size, below 2^32
+  int64_t d_ps;
+  FastDiv fd_page;
 };
+
+// The destination row (elements) of row n of layer l at slot `slot`.
+__device__ __forceinline__ int64_t paged_row(const CommitArgs& a, int64_t l, int64_t slot) {
+  const uint32_t s = static_cast<uint32_t>(slot);
+  const uint32_t page = fdiv(s, a.fd_page);
+  return l * a.d_ls + static_cast<int64_t>(page) * a.d_ps +
+         static_cast<int64_t>(s - page * a.fd_page.d) * a.d_ts;
+}
 
 // The pair rotation with torch's rounding sequence.
 __device__ __forceinline__ void rope_pair(float x0, float x1, float c0, float s0, float c1,
@@ -57,8 +75,9 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c0, float s0
 }
 
 // KV2: K rows and V rows on separate waves, all K waves first (each wave
-// streams one tensor; a V wave is a plain copy and reads no table).
-template <class Tag, int CH, bool KV2>
+// streams one tensor; a V wave is a plain copy and reads no table). PAGED: rows
+// go where slots says. ROPE false: K is copied.
+template <class Tag, int CH, bool KV2, bool PAGED = false, bool ROPE = true>
 __global__ __launch_bounds__(kBlock) void rope_commit_kernel(const CommitArgs a) {
   static_assert(Tag::kVec == 8, "16-bit rows");
   const int lane = threadIdx.x % kWave;
@@ -78,7 +97,10 @@ __global__ __launch_bounds__(kBlock) void rope_commit_kernel(const CommitArgs a)
   const int64_t b = lb32 - l32 * static_cast<uint32_t>(a.batch);
   const int64_t l = l32;
   const int64_t so = l * a.s_ls + b * a.s_bs + n * a.s_ts;
-  const int64_t dof = l * a.d_ls + b * a.d_bs + (a.d_off + n) * a.d_ts;
+  int64_t slot = 0;
+  if constexpr (PAGED) slot = a.slots[n];
+  int64_t dof = 0;
+  if constexpr (!PAGED) dof = l * a.d_ls + b * a.d_bs + (a.d_off + n) * a.d_ts;
   const bool do_k = !v_wave;
   const bool do_v = a.src_v != nullptr && (!KV2 || v_wave);
 
@@ -89,14 +111,16 @@ __global__ __launch_bounds__(kBlock) void rope_commit_kernel(const CommitArgs a)
   u32x4 k[CH], v[CH];
   u32x4 c_lo, c_hi, s_lo, s_hi;
   if (do_k) {
-    // Table columns of this lane (same in every chunk: 512 % D == 0).
-    const int d0 = (lane * 8) % a.head_dim;
-    const float* ct = a.cos + b * a.tab_bs + n * a.tab_ts + d0;
-    const float* st = a.sin + b * a.tab_bs + n * a.tab_ts + d0;
-    c_lo = ld16(ct);
-    c_hi = ld16(ct + 4);
-    s_lo = ld16(st);
-    s_hi = ld16(st + 4);
+    if constexpr (ROPE) {
+      // Table columns of this lane (same in every chunk: 512 % D == 0).
+      const int d0 = (lane * 8) % a.head_dim;
+      const float* ct = a.cos + b * a.tab_bs + n * a.tab_ts + d0;
+      const float* st = a.sin + b * a.tab_bs + n * a.tab_ts + d0;
+      c_lo = ld16(ct);
+      c_hi = ld16(ct + 4);
+      s_lo = ld16(st);
+      s_hi = ld16(st + 4);
+    }
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int e = i * 512 + lane * 8;
@@ -110,7 +134,18 @@ __global__ __launch_bounds__(kBlock) void rope_commit_kernel(const CommitArgs a)
       v[i] = ld16_nt(byte_off(a.src_v, (so + (e < a.row_elems ? e : e_safe)) * Tag::kBytes));
     }
   }
-  if (do_k) {
+  if constexpr (PAGED) {
+    if (slot < 0 || slot >= a.n_slots) return;  // uniform over the wave
+    dof = paged_row(a, l, slot);
+  }
+  if (do_k && !ROPE) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int e = i * 512 + lane * 8;
+      if (e < a.row_elems) st16_nt(byte_off(a.dst_k, (dof + e) * Tag::kBytes), k[i]);
+    }
+  }
+  if (do_k && ROPE) {
     float cs[8], sn[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -141,7 +176,7 @@ __global__ __launch_bounds__(kBlock) void rope_commit_kernel(const CommitArgs a)
 }
 
 // One row per workgroup, element pairs (any head_dim, any alignment).
-template <class Tag>
+template <class Tag, bool PAGED = false>
 __global__ __launch_bounds__(kBlock) void rope_commit_generic_kernel(const CommitArgs a) {
   const int64_t row = blockIdx.x;
   const int64_t n = row % a.tokens;
@@ -149,15 +184,22 @@ __global__ __launch_bounds__(kBlock) void rope_commit_generic_kernel(const Commi
   const int64_t b = lb % a.batch;
   const int64_t l = lb / a.batch;
   const int64_t so = l * a.s_ls + b * a.s_bs + n * a.s_ts;
-  const int64_t dof = l * a.d_ls + b * a.d_bs + (a.d_off + n) * a.d_ts;
+  int64_t dof;
+  if constexpr (PAGED) {
+    const int64_t slot = a.slots[n];
+    if (slot < 0 || slot >= a.n_slots) return;
+    dof = paged_row(a, l, slot);
+  } else {
+    dof = l * a.d_ls + b * a.d_bs + (a.d_off + n) * a.d_ts;
+  }
   const float* ct = a.cos + b * a.tab_bs + n * a.tab_ts;
   const float* st = a.sin + b * a.tab_bs + n * a.tab_ts;
   for (int p = threadIdx.x; p < a.row_elems / 2; p += kBlock) {
     const int e = 2 * p;
     const int d = e % a.head_dim;
-    float o0, o1;
-    rope_pair(load_elem<Tag>(a.src_k, so + e), load_elem<Tag>(a.src_k, so + e + 1), ct[d], st[d],
-              ct[d + 1], st[d + 1], o0, o1);
+    float o0 = load_elem<Tag>(a.src_k, so + e), o1 = load_elem<Tag>(a.src_k, so + e + 1);
+    if (!PAGED || a.cos != nullptr)
+      rope_pair(o0, o1, ct[d], st[d], ct[d + 1], st[d + 1], o0, o1);
     store_elem<Tag>(a.dst_k, dof + e, o0);
     store_elem<Tag>(a.dst_k, dof + e + 1, o1);
     if (a.src_v) {
@@ -167,7 +209,7 @@ __global__ __launch_bounds__(kBlock) void rope_commit_generic_kernel(const Commi
   }
 }
 
-template <class Tag>
+template <class Tag, bool PAGED = false, bool ROPE = true>
 int launch_commit(const CommitArgs& args, hipStream_t stream) {
   CommitArgs a = args;
   a.fd_tokens = make_fastdiv(static_cast<uint32_t>(a.tokens));
@@ -182,7 +224,7 @@ int launch_commit(const CommitArgs& args, hipStream_t stream) {
                       al(a.src_v, a.s_ls) && al(a.src_v, a.s_bs) && al(a.src_v, a.s_ts) &&
                       al(a.dst_k, a.d_ls) && al(a.dst_k, a.d_bs) && al(a.dst_k, a.d_ts) &&
                       al(a.dst_v, a.d_ls) && al(a.dst_v, a.d_bs) && al(a.dst_v, a.d_ts) &&
-                      aligned(a.cos, 16) && aligned(a.sin, 16) && a.tab_ts % 4 == 0 &&
+                      al(a.dst_k, a.d_ps) && al(a.dst_v, a.d_ps) && aligned(a.cos, 16) && aligned(a.sin, 16) && a.tab_ts % 4 == 0 &&
                       a.tab_bs % 4 == 0;
   const int chunks = (a.row_elems + 511) / 512;
   // K and V on separate waves: 40 x 1560 x [32, 128] 357 -> 340 us (twice the
@@ -194,9 +236,9 @@ int launch_commit(const CommitArgs& args, hipStream_t stream) {
   auto go = [&](auto ch) {
     constexpr int CH = decltype(ch)::value;
     if (kv2)
-      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, true>), grid, dim3(kBlock), 0, stream, a);
+      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, true, PAGED, ROPE>), grid, dim3(kBlock), 0, stream, a);
     else
-      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, false>), grid, dim3(kBlock), 0, stream, a);
+      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, false, PAGED, ROPE>), grid, dim3(kBlock), 0, stream, a);
   };
   if (vec_ok && chunks <= 1)
     go(std::integral_constant<int, 1>{});
@@ -211,9 +253,9 @@ int launch_commit(const CommitArgs& args, hipStream_t stream) {
   else
     launched = false;
   if (!launched)
-    hipLaunchKernelGGL((rope_commit_generic_kernel<Tag>), dim3(static_cast<unsigned>(rows)),
+    hipLaunchKernelGGL((rope_commit_generic_kernel<Tag, PAGED>), dim3(static_cast<unsigned>(rows)),
                        dim3(kBlock), 0, stream, a);
-  return launch_status("kv_commit_rope");
+  return launch_status(PAGED ? "kv_commit_rope_paged" : "kv_commit_rope");
 }
 
 }  // namespace
@@ -263,4 +305,49 @@ extern "C" int jo_kv_commit_rope(const void* src_k, const void* src_v, void* dst
                table_batch_stride};
   hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == JO_DTYPE_BF16 ? launch_commit<BF16>(a, st) : launch_commit<F16>(a, st);
+}
+
+extern "C" int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, void* pages_k,
+                                       void* pages_v, int64_t layers, int64_t tokens,
+                                       int64_t num_heads, int64_t head_dim,
+                                       int64_t src_layer_stride, int64_t src_token_stride,
+                                       int64_t pages_layer_stride, int64_t page_stride,
+                                       int64_t pages_token_stride, int64_t num_pages,
+                                       int64_t page_size, const int64_t* slots, const float* cos,
+                                       const float* sin, int64_t table_stride, int dtype,
+                                       void* stream) {
+  const char* op = "kv_commit_rope_paged";
+  JO_REQUIRE(dtype == JO_DTYPE_BF16 || dtype == JO_DTYPE_F16, "%s: K/V must be bf16 or fp16", op);
+  JO_REQUIRE(layers >= 0 && tokens >= 0 && num_heads > 0 && head_dim > 0 && num_pages >= 0,
+             "%s: bad shape", op);
+  JO_REQUIRE(page_size >= 1 && page_size <= INT32_MAX && num_pages <= UINT32_MAX / page_size,
+             "%s: bad page_size, or a pool of 2^32 tokens and more", op);
+  JO_REQUIRE(head_dim % 2 == 0, "%s: an even head dimension is needed, got %lld", op,
+             static_cast<long long>(head_dim));
+  JO_REQUIRE(num_heads <= INT32_MAX / 2 / head_dim, "%s: row too long", op);
+  JO_REQUIRE((cos == nullptr) == (sin == nullptr), "%s: cos and sin go together", op);
+  JO_REQUIRE(src_token_stride >= num_heads * head_dim && src_layer_stride >= 0 &&
+                 pages_token_stride >= num_heads * head_dim && page_stride >= 0 &&
+                 pages_layer_stride >= 0 && (cos == nullptr || table_stride >= head_dim),
+             "%s: bad stride", op);
+  JO_REQUIRE(layers == 0 || tokens <= INT64_MAX / layers, "%s: too many rows", op);
+  const int64_t rows = layers * tokens;
+  if (rows == 0 || num_pages == 0) return JO_OK;  // nothing to write, or nowhere
+  JO_REQUIRE((src_v == nullptr) == (pages_v == nullptr),
+             "%s: V needs both a source and a destination", op);
+  JO_REQUIRE(rows <= int64_t{UINT32_MAX} / (2 * 64), "%s: too many rows (%lld, at most %lld)", op,
+             static_cast<long long>(rows), static_cast<long long>(int64_t{UINT32_MAX} / (2 * 64)));
+  JO_REQUIRE(src_k && pages_k && slots, "%s: null pointer", op);
+  CommitArgs a{src_k, src_v, pages_k, pages_v, layers, 1, tokens,
+               static_cast<int>(num_heads * head_dim), static_cast<int>(head_dim),
+               src_layer_stride, 0, src_token_stride, pages_layer_stride, 0, pages_token_stride, 0,
+               cos, sin, cos ? table_stride : 0, 0};
+  a.slots = slots;
+  a.n_slots = num_pages * page_size;
+  a.d_ps = page_stride;
+  a.fd_page = make_fastdiv(static_cast<uint32_t>(page_size));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == JO_DTYPE_BF16)
+    return cos ? launch_commit<BF16, true, true>(a, st) : launch_commit<BF16, true, false>(a, st);
+  return cos ? launch_commit<F16, true, true>(a, st) : launch_commit<F16, true, false>(a, st);
 }

@@ -7,7 +7,8 @@
 // torch.ops.joyomni_ops.* behaves as the reference does for callers. The new
 // ops (grid RoPE, K ring-cache write, QK with the pre-RoPE K stage,
 // add+LayerNorm, RMSNorm->FP8, norm+AdaLN->FP8, KV-pool commit,
-// apply_rotary_emb, per-head RMSNorm) have their own names. Tensors on ROCm
+// apply_rotary_emb, per-head RMSNorm, the paged KV tables and commit, attention
+// over pages and packed prompts) have their own names. Tensors on ROCm
 // carry the CUDA device type, so the impls are registered on the CUDA
 // dispatch key like the reference's. Every op runs
 // on the current stream of the tensor's device and never synchronizes.
@@ -16,6 +17,7 @@
 #include <torch/all.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <vector>
 
 #include "joyomni_hip.h"
@@ -1037,6 +1039,301 @@ void qk_norm_rope_kstage(torch::Tensor& q, torch::Tensor& k, torch::Tensor& k_st
   fused_qk_norm_rope_3d_paired_kstage(q, k, k_stage, L, H, eps, q_weight, k_weight, c, s);
 }
 
+// ---------------------------------------------------------------------------
+// Serving over a paged KV pool.
+// ---------------------------------------------------------------------------
+namespace {
+// An int32 array of the step's tables on the device of the step's tensors.
+void check_i32(const torch::Tensor& t, const torch::Device& dev, const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", is on ", t.device());
+  TORCH_CHECK(t.scalar_type() == torch::kInt32, name, " must be int32");
+}
+void check_i32_vector(const torch::Tensor& t, const torch::Device& dev, const char* name) {
+  check_i32(t, dev, name);
+  TORCH_CHECK(t.dim() == 1 && (t.numel() <= 1 || t.stride(0) == 1), name,
+              " must be 1D contiguous");
+}
+// The block table [requests, width]; returns its row stride.
+int64_t check_table(const torch::Tensor& t, const torch::Device& dev, int64_t requests) {
+  check_i32(t, dev, "block_table");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == requests, "block_table must be [requests, width]");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, "block_table must have contiguous rows");
+  return row_stride(t);
+}
+}  // namespace
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> paged_tables(
+    const torch::Tensor& ctx_lens, const torch::Tensor& new_lens, torch::Tensor block_table,
+    const torch::Tensor& free_pages, const torch::Tensor& num_free, int64_t page_size,
+    int64_t num_pages, int64_t max_tokens) {
+  JO_CHECK_CUDA(ctx_lens);
+  const torch::Device dev = ctx_lens.device();
+  check_i32_vector(ctx_lens, dev, "ctx_lens");
+  check_i32_vector(new_lens, dev, "new_lens");
+  check_i32_vector(free_pages, dev, "free_pages");
+  check_i32_vector(num_free, dev, "num_free");
+  const int64_t R = ctx_lens.size(0);
+  TORCH_CHECK(new_lens.size(0) == R, "ctx_lens and new_lens must have the same length");
+  TORCH_CHECK(num_free.numel() == 1, "num_free must hold one number");
+  const int64_t ts = check_table(block_table, dev, R);
+  TORCH_CHECK(max_tokens >= 0 && max_tokens <= INT32_MAX, "max_tokens must be in [0, 2^31)");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+  auto cu = torch::empty({R + 1}, ctx_lens.options());
+  auto kv = torch::empty({R}, ctx_lens.options());
+  auto slots = torch::empty({max_tokens}, ctx_lens.options().dtype(torch::kInt64));
+  auto left = torch::empty({1}, ctx_lens.options());
+  check_status(
+      jo_paged_tables(ctx_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), R,
+                      block_table.data_ptr<int32_t>(), ts, block_table.size(1),
+                      free_pages.data_ptr<int32_t>(), free_pages.numel(),
+                      num_free.data_ptr<int32_t>(), page_size, num_pages, max_tokens,
+                      cu.data_ptr<int32_t>(), kv.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
+                      left.data_ptr<int32_t>(), current_stream(ctx_lens)),
+      "paged_tables");
+  return {cu, kv, slots, left};
+}
+
+void kv_commit_rope_paged(const torch::Tensor& src_k, const c10::optional<torch::Tensor>& src_v,
+                          torch::Tensor pages_k, const c10::optional<torch::Tensor>& pages_v,
+                          const torch::Tensor& slots, const c10::optional<torch::Tensor>& cos,
+                          const c10::optional<torch::Tensor>& sin) {
+  JO_CHECK_CUDA(src_k);
+  const torch::Device dev = src_k.device();
+  TORCH_CHECK(src_k.dim() == 3 || src_k.dim() == 4, "src_k must be [T, H, D] or [L, T, H, D]");
+  TORCH_CHECK(src_k.scalar_type() == torch::kBFloat16 || src_k.scalar_type() == torch::kFloat16,
+              "src_k must be bf16 or fp16");
+  const int64_t o = src_k.dim() - 3;  // 1: with layers
+  const int64_t L = o ? src_k.size(0) : 1, T = src_k.size(o), H = src_k.size(o + 1),
+                D = src_k.size(o + 2);
+  auto rows = [&](const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", is on ", t.device());
+    TORCH_CHECK(t.scalar_type() == src_k.scalar_type(), name, " must have src_k's dtype");
+    TORCH_CHECK((D <= 1 || t.stride(-1) == 1) && (H <= 1 || t.stride(-2) == D), name,
+                " must have contiguous heads per token");
+  };
+  rows(src_k, "src_k");
+  rows(pages_k, "pages_k");
+  TORCH_CHECK(pages_k.dim() == src_k.dim() + 1 && (!o || pages_k.size(0) == L) &&
+                  pages_k.size(-2) == H && pages_k.size(-1) == D,
+              "pages_k must be [N, P, H, D] ([L, N, P, H, D] with layers) with src_k's heads");
+  const int64_t N = pages_k.size(o), P = pages_k.size(o + 1);
+  TORCH_CHECK(P >= 1, "pages must hold at least one token");
+  // A size-1 dim's stride is never used to move: report the dense one.
+  auto token_stride = [&](const torch::Tensor& t) {
+    return t.size(-3) <= 1 ? H * D : t.stride(-3);
+  };
+  auto page_stride = [&](const torch::Tensor& t) { return N <= 1 ? P * H * D : t.stride(o); };
+  auto layer_stride = [&](const torch::Tensor& t) { return L <= 1 ? 0 : t.stride(0); };
+  const bool has_v = src_v.has_value() && src_v->defined();
+  TORCH_CHECK(has_v == (pages_v.has_value() && pages_v->defined()),
+              "src_v and pages_v go together");
+  if (has_v) {
+    rows(*src_v, "src_v");
+    rows(*pages_v, "pages_v");
+    TORCH_CHECK(src_v->sizes() == src_k.sizes() && pages_v->sizes() == pages_k.sizes() &&
+                    token_stride(*src_v) == token_stride(src_k) &&
+                    layer_stride(*src_v) == layer_stride(src_k) &&
+                    token_stride(*pages_v) == token_stride(pages_k) &&
+                    page_stride(*pages_v) == page_stride(pages_k) &&
+                    layer_stride(*pages_v) == layer_stride(pages_k),
+                "V tensors must have the shapes and strides of the K tensors");
+  }
+  TORCH_CHECK(slots.device() == dev && slots.scalar_type() == torch::kInt64 && slots.dim() == 1 &&
+                  slots.size(0) == T && (T <= 1 || slots.stride(0) == 1),
+              "slots must be a contiguous int64 [T] on src_k's device");
+  const bool rope = cos.has_value() && cos->defined();
+  TORCH_CHECK(rope == (sin.has_value() && sin->defined()), "cos and sin go together");
+  if (rope)
+    for (const torch::Tensor* t : {&*cos, &*sin})
+      TORCH_CHECK(t->device() == dev && t->scalar_type() == torch::kFloat32 &&
+                      t->is_contiguous() && t->dim() == 2 && t->size(0) == T && t->size(1) == D,
+                  "cos and sin must be contiguous float32 [T, D] on src_k's device");
+  if (src_k.numel() == 0) return;
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+  check_status(jo_kv_commit_rope_paged(
+                   src_k.data_ptr(), has_v ? src_v->data_ptr() : nullptr, pages_k.data_ptr(),
+                   has_v ? pages_v->data_ptr() : nullptr, L, T, H, D, layer_stride(src_k),
+                   token_stride(src_k), layer_stride(pages_k), page_stride(pages_k),
+                   token_stride(pages_k), N, P, slots.data_ptr<int64_t>(),
+                   rope ? cos->data_ptr<float>() : nullptr,
+                   rope ? sin->data_ptr<float>() : nullptr, D, dtype_code(src_k),
+                   current_stream(src_k)),
+               "kv_commit_rope_paged");
+}
+
+namespace {
+// A [tokens, heads, D] tensor of the attention ops (pages: [N, P, heads, D]) as
+// the kernels read it: D contiguous, other strides multiples of 8 elements, the
+// start 16-byte aligned. A dim of one is given stride 0.
+struct AttnRows {
+  int64_t ps, ts, hs;  // page, token, head
+};
+AttnRows attn_rows(const torch::Tensor& t, const torch::Tensor& q, int dims, const char* name) {
+  TORCH_CHECK(t.device() == q.device(), name, " must be on ", q.device(), ", is on ", t.device());
+  TORCH_CHECK(t.scalar_type() == q.scalar_type(), name, " must have q's dtype");
+  TORCH_CHECK(t.dim() == dims && t.size(dims - 1) == q.size(2), name, " must be ",
+              dims == 3 ? "[tokens, heads, head_dim]" : "[pages, page_size, heads, head_dim]",
+              " with q's head_dim");
+  auto stride = [&](int d) { return t.size(d) <= 1 ? 0 : t.stride(d); };
+  const AttnRows r{dims == 4 ? stride(0) : 0, stride(dims - 3), stride(dims - 2)};
+  if (t.numel() > 0)
+    TORCH_CHECK(t.stride(dims - 1) == 1 && r.ps % 8 == 0 && r.ts % 8 == 0 && r.hs % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                name, " must have a contiguous head_dim, strides that are multiples of 8 "
+                "elements and a 16-byte aligned start");
+  return r;
+}
+
+// First and one-past-last byte that a tensor's elements touch.
+std::pair<uintptr_t, uintptr_t> byte_range(const torch::Tensor& t) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + static_cast<uintptr_t>((last + 1) * t.element_size())};
+}
+
+struct AttnCall {
+  int64_t T, Hq, Hkv, D, R;
+  AttnRows q, k, v, o;
+  double scale;
+  int dtype;
+  torch::Tensor ws;
+  int64_t ws_bytes;
+};
+
+AttnCall attn_check(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                    int kv_dims, const torch::Tensor& cu_q, c10::optional<double> scale,
+                    const torch::Tensor& out) {
+  AttnCall c;
+  TORCH_CHECK(q.scalar_type() == torch::kBFloat16 || q.scalar_type() == torch::kFloat16,
+              "q must be bf16 or fp16");
+  c.T = q.size(0), c.Hq = q.size(1), c.D = q.size(2);
+  TORCH_CHECK(c.D == 64 || c.D == 128 || c.D == 256, "Unsupported head_dim: ", c.D);
+  c.q = attn_rows(q, q, 3, "q");
+  c.k = attn_rows(k, q, kv_dims, kv_dims == 3 ? "k" : "pages_k");
+  c.v = attn_rows(v, q, kv_dims, kv_dims == 3 ? "v" : "pages_v");
+  TORCH_CHECK(v.sizes() == k.sizes(), "the value tensor must have the key tensor's shape");
+  c.Hkv = k.size(kv_dims - 2);
+  TORCH_CHECK(c.Hkv > 0 && c.Hq > 0 && c.Hq % c.Hkv == 0,
+              "q's heads (", c.Hq, ") must be a multiple of the key heads (", c.Hkv, ")");
+  check_i32_vector(cu_q, q.device(), "cu_q");
+  TORCH_CHECK(cu_q.numel() >= 1, "cu_q must be [requests + 1]");
+  c.R = cu_q.numel() - 1;
+  c.o = attn_rows(out, q, 3, "out");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  c.scale = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(c.D));
+  c.dtype = dtype_code(q);
+  return c;
+}
+
+// An `out` of the caller's own, written while inputs are still being read.
+void attn_no_overlap(const torch::Tensor& out, std::initializer_list<const torch::Tensor*> in) {
+  if (out.numel() == 0) return;
+  const auto a = byte_range(out);
+  for (const torch::Tensor* t : in) {
+    if (t->numel() == 0) continue;
+    const auto b = byte_range(*t);
+    TORCH_CHECK(a.second <= b.first || b.second <= a.first, "out must not overlap an input");
+  }
+}
+
+void attn_workspace(AttnCall& c, const torch::Tensor& q, int64_t kv_capacity) {
+  c.ws_bytes = jo_attention_workspace_bytes(c.T, c.R, c.Hq, c.Hkv, c.D, kv_capacity);
+  if (c.ws_bytes > 0) c.ws = torch::empty({c.ws_bytes}, q.options().dtype(torch::kUInt8));
+}
+
+void run_varlen(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                const torch::Tensor& cu_q, const c10::optional<torch::Tensor>& cu_k,
+                c10::optional<double> scale, bool causal, const torch::Tensor& out, bool fill) {
+  AttnCall c = attn_check(q, k, v, 3, cu_q, scale, out);
+  const bool own_k = cu_k.has_value() && cu_k->defined();
+  if (own_k) {
+    check_i32_vector(*cu_k, q.device(), "cu_k");
+    TORCH_CHECK(cu_k->numel() == cu_q.numel(), "cu_k must have cu_q's length");
+  } else {
+    TORCH_CHECK(k.size(0) == c.T, "k must have q's tokens when cu_k is not given");
+  }
+  if (q.numel() == 0) return;
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  attn_workspace(c, q, k.size(0));
+  check_status(jo_attention_varlen(
+                   q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), c.T, k.size(0), c.R,
+                   c.Hq, c.Hkv, c.D, c.q.ts, c.q.hs, c.k.ts, c.k.hs, c.v.ts, c.v.hs, c.o.ts,
+                   c.o.hs, cu_q.data_ptr<int32_t>(),
+                   (own_k ? *cu_k : cu_q).data_ptr<int32_t>(), static_cast<float>(c.scale), causal,
+                   fill, c.dtype, c.ws_bytes > 0 ? c.ws.data_ptr() : nullptr, c.ws_bytes,
+                   current_stream(q)),
+               "attention_varlen");
+}
+
+void run_paged(const torch::Tensor& q, const torch::Tensor& pages_k, const torch::Tensor& pages_v,
+               const torch::Tensor& block_table, const torch::Tensor& cu_q,
+               const torch::Tensor& kv_lens, c10::optional<double> scale, bool causal,
+               const torch::Tensor& out, bool fill) {
+  AttnCall c = attn_check(q, pages_k, pages_v, 4, cu_q, scale, out);
+  const int64_t N = pages_k.size(0), P = pages_k.size(1);
+  TORCH_CHECK(P >= 1, "pages must hold at least one token");
+  const int64_t ts = check_table(block_table, q.device(), c.R), W = block_table.size(1);
+  check_i32_vector(kv_lens, q.device(), "kv_lens");
+  TORCH_CHECK(kv_lens.numel() == c.R, "kv_lens must be [requests]");
+  if (q.numel() == 0) return;
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  attn_workspace(c, q, W * P);
+  check_status(jo_attention_paged(
+                   q.data_ptr(), pages_k.data_ptr(), pages_v.data_ptr(), out.data_ptr(), c.T, c.R,
+                   c.Hq, c.Hkv, c.D, N, P, c.q.ts, c.q.hs, c.k.ps, c.k.ts, c.k.hs, c.v.ps, c.v.ts,
+                   c.v.hs, c.o.ts, c.o.hs, block_table.data_ptr<int32_t>(), ts, W,
+                   cu_q.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                   static_cast<float>(c.scale), causal, fill, c.dtype,
+                   c.ws_bytes > 0 ? c.ws.data_ptr() : nullptr, c.ws_bytes, current_stream(q)),
+               "attention_paged");
+}
+
+torch::Tensor attn_out(const torch::Tensor& q) {
+  JO_CHECK_CUDA(q);
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
+  return torch::empty(q.sizes(), q.options());
+}
+}  // namespace
+
+torch::Tensor attention_varlen(const torch::Tensor& q, const torch::Tensor& k,
+                               const torch::Tensor& v, const torch::Tensor& cu_q,
+                               const c10::optional<torch::Tensor>& cu_k,
+                               c10::optional<double> scale, bool causal) {
+  auto out = attn_out(q);
+  run_varlen(q, k, v, cu_q, cu_k, scale, causal, out, true);
+  return out;
+}
+
+void attention_varlen_out(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                          const torch::Tensor& cu_q, const c10::optional<torch::Tensor>& cu_k,
+                          c10::optional<double> scale, bool causal, torch::Tensor out) {
+  JO_CHECK_CUDA(q);
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
+  attn_no_overlap(out, {&q, &k, &v, &cu_q});
+  run_varlen(q, k, v, cu_q, cu_k, scale, causal, out, false);
+}
+
+torch::Tensor attention_paged(const torch::Tensor& q, const torch::Tensor& pages_k,
+                              const torch::Tensor& pages_v, const torch::Tensor& block_table,
+                              const torch::Tensor& cu_q, const torch::Tensor& kv_lens,
+                              c10::optional<double> scale, bool causal) {
+  auto out = attn_out(q);
+  run_paged(q, pages_k, pages_v, block_table, cu_q, kv_lens, scale, causal, out, true);
+  return out;
+}
+
+void attention_paged_out(const torch::Tensor& q, const torch::Tensor& pages_k,
+                         const torch::Tensor& pages_v, const torch::Tensor& block_table,
+                         const torch::Tensor& cu_q, const torch::Tensor& kv_lens,
+                         c10::optional<double> scale, bool causal, torch::Tensor out) {
+  JO_CHECK_CUDA(q);
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
+  attn_no_overlap(out, {&q, &pages_k, &pages_v, &block_table, &cu_q, &kv_lens});
+  run_paged(q, pages_k, pages_v, block_table, cu_q, kv_lens, scale, causal, out, false);
+}
+
 }  // namespace joyomni_ops
 
 TORCH_LIBRARY(joyomni_ops, m) {
@@ -1116,6 +1413,25 @@ TORCH_LIBRARY(joyomni_ops, m) {
   m.def(
       "qk_norm_rope_kstage(Tensor(a!) q, Tensor(b!) k, Tensor(c!) k_stage, float eps, "
       "Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin) -> ()");
+  m.def(
+      "paged_tables(Tensor ctx_lens, Tensor new_lens, Tensor(a!) block_table, Tensor free_pages, "
+      "Tensor num_free, int page_size, int num_pages, int max_tokens) "
+      "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "kv_commit_rope_paged(Tensor src_k, Tensor? src_v, Tensor(a!) pages_k, Tensor(b!)? pages_v, "
+      "Tensor slots, Tensor? cos, Tensor? sin) -> ()");
+  m.def(
+      "attention_varlen(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor? cu_k, float? scale, "
+      "bool causal) -> Tensor");
+  m.def(
+      "attention_varlen_out(Tensor q, Tensor k, Tensor v, Tensor cu_q, Tensor? cu_k, "
+      "float? scale, bool causal, Tensor(a!) out) -> ()");
+  m.def(
+      "attention_paged(Tensor q, Tensor pages_k, Tensor pages_v, Tensor block_table, Tensor cu_q, "
+      "Tensor kv_lens, float? scale, bool causal) -> Tensor");
+  m.def(
+      "attention_paged_out(Tensor q, Tensor pages_k, Tensor pages_v, Tensor block_table, "
+      "Tensor cu_q, Tensor kv_lens, float? scale, bool causal, Tensor(a!) out) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(joyomni_ops, CUDA, m) {
@@ -1148,6 +1464,12 @@ TORCH_LIBRARY_IMPL(joyomni_ops, CUDA, m) {
   m.impl("qk_norm_rope_inplace", &joyomni_ops::qk_norm_rope_inplace);
   m.impl("qk_norm_rope_copies", &joyomni_ops::qk_norm_rope_copies);
   m.impl("qk_norm_rope_kstage", &joyomni_ops::qk_norm_rope_kstage);
+  m.impl("paged_tables", &joyomni_ops::paged_tables);
+  m.impl("kv_commit_rope_paged", &joyomni_ops::kv_commit_rope_paged);
+  m.impl("attention_varlen", &joyomni_ops::attention_varlen);
+  m.impl("attention_varlen_out", &joyomni_ops::attention_varlen_out);
+  m.impl("attention_paged", &joyomni_ops::attention_paged);
+  m.impl("attention_paged_out", &joyomni_ops::attention_paged_out);
 }
 
 // Ops that allocate results which autograd never saw: the ops that they call

@@ -14,7 +14,9 @@ fused_qk_norm_rope_3d_grid_kstage, fused_qk_norm_rope_3d_tables,
 fused_qk_norm_rope_3d_tables_kstage, fused_add_layernorm_scale_shift,
 rmsnorm_quant_fp8, norm_scale_shift_quant_fp8, kv_commit_rope,
 apply_rotary_emb, rmsnorm_heads, gelu_tanh_quant_fp8,
-fused_norm_scale_shift_per_sample, plus rope_freqs() to build the
+fused_norm_scale_shift_per_sample, and for serving many streams from one paged
+KV pool paged_tables, kv_commit_rope_paged, attention_paged and
+attention_varlen, plus rope_freqs() to build the
 [2, head_dim/2] frequency table the grid ops read.
 """
 from __future__ import annotations
@@ -58,6 +60,10 @@ __all__ = [
     "fused_qk_norm_rope_3d_tables_kstage",
     "gelu_tanh_quant_fp8",
     "fused_norm_scale_shift_per_sample",
+    "paged_tables",
+    "kv_commit_rope_paged",
+    "attention_paged",
+    "attention_varlen",
 ]
 
 _ops = torch.ops.joyomni_ops
@@ -293,3 +299,82 @@ def rmsnorm_heads(x, weight, eps=1e-6, round_first=False):
     rmsnorm kernel (rmsnorm.cu:57-60). round_first=True: the torch RMSNorm
     module, round(round(x * r) * w) (dit.py:244-249)."""
     return _ops.rmsnorm_heads(x, weight, eps, 1 if round_first else 0)
+
+
+# ---------------------------------------------------------------------------
+# Serving many streams from one paged KV pool.
+# ---------------------------------------------------------------------------
+def paged_tables(ctx_lens, new_lens, block_table, free_pages, num_free, page_size, num_pages,
+                 max_tokens):
+    """The tables of a serving step, built on the GPU from its request lengths.
+
+    ctx_lens, new_lens: int32 [R], tokens already cached and tokens of this
+    step; block_table: int32 [R, W], updated in place with the pages that the
+    step's tokens newly need; free_pages: int32 stack of free page ids, of which
+    the first num_free (int32 [1]) count; max_tokens: the step's fixed size.
+    Returns (cu_q int32 [R + 1], kv_lens int32 [R], slots int64 [max_tokens],
+    free_left int32 [1]): where each request's tokens begin, its keys after the
+    step, the pool place of each token's K and V (page * page_size + place, -1
+    where there is none: padding, or the pages ran out), and num_free for the
+    next step (negative: that many pages are missing). The stack is only read.
+    """
+    return _ops.paged_tables(ctx_lens, new_lens, block_table, free_pages, num_free, page_size,
+                             num_pages, max_tokens)
+
+
+def kv_commit_rope_paged(src_k, pages_k, slots, cos=None, sin=None, src_v=None, pages_v=None):
+    """kv_commit_rope into pages: K row n, rotated by cos[n], sin[n] (fp32 [T, D];
+    as it is without them), and V row n go to place slots[n] % page_size of page
+    slots[n] // page_size, for every layer in one launch. A slot outside the pool
+    (paged_tables' -1) leaves its row out; slots of one call must differ.
+    src: [T, H, D] or [L, T, H, D]; pages: [N, P, H, D] or [L, N, P, H, D]."""
+    _ops.kv_commit_rope_paged(src_k, src_v, pages_k, pages_v, slots, cos, sin)
+
+
+def attention_paged(q, pages_k, pages_v, block_table, cu_q, kv_lens, causal=True, scale=None,
+                    out=None):
+    """Attention of each request's new tokens over its keys in the pages.
+
+    q: bf16 / fp16 [T, Hq, D] (D 64, 128 or 256), request r's tokens at
+    cu_q[r] .. cu_q[r + 1] - 1 (int32 [R + 1]): a single token, a chunk, or none;
+    pages: [N, P, Hkv, D], Hq a multiple of Hkv; block_table: int32 [R, W];
+    kv_lens: int32 [R], keys of each request, the new tokens' own among them.
+    causal: a request's last token sees all its keys, the one before it all but
+    the last, and so on; otherwise every token sees every key. scale: 1/sqrt(D)
+    when None. Tokens that see nothing get zeros.
+    Returns a new [T, Hq, D] tensor with zeros behind the last request, or writes
+    `out` (rows behind the last request stay as they are) and returns it.
+    """
+    if out is None:
+        return _ops.attention_paged(q, pages_k, pages_v, block_table, cu_q, kv_lens, scale, causal)
+    _ops.attention_paged_out(q, pages_k, pages_v, block_table, cu_q, kv_lens, scale, causal, out)
+    return out
+
+
+def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
+    """Attention over sequences packed one behind the other, each with itself.
+
+    q: bf16 / fp16 [T, Hq, D], sequence r at cu_q[r] .. cu_q[r + 1] - 1; k, v:
+    [Tk, Hkv, D], at cu_k[r] .. cu_k[r + 1] - 1 (cu_q when None: self-attention).
+    Token and head strides are free (multiples of 8 elements), so q, k and v can
+    be slices of a packed projection. causal, scale, out and the result as in
+    attention_paged (causal=False is the DiT's attention).
+    """
+    if out is None:
+        return _ops.attention_varlen(q, k, v, cu_q, cu_k, scale, causal)
+    _ops.attention_varlen_out(q, k, v, cu_q, cu_k, scale, causal, out)
+    return out
+
+
+# Shapes of the results, for tracing.
+@torch.library.register_fake("joyomni_ops::paged_tables")
+def _(ctx_lens, new_lens, block_table, free_pages, num_free, page_size, num_pages, max_tokens):
+    n = ctx_lens.shape[0]
+    return (ctx_lens.new_empty(n + 1), ctx_lens.new_empty(n),
+            ctx_lens.new_empty(max_tokens, dtype=torch.int64), ctx_lens.new_empty(1))
+
+
+@torch.library.register_fake("joyomni_ops::attention_paged")
+@torch.library.register_fake("joyomni_ops::attention_varlen")
+def _(q, *args):
+    return q.new_empty(q.shape)

@@ -45,7 +45,7 @@ _I64 = c_int64
 _F = c_float
 
 # Entry points that return something other than an int status.
-RESTYPES = {"jo_fp8_scaled_mm_workspace_bytes": _I64}
+RESTYPES = {"jo_fp8_scaled_mm_workspace_bytes": _I64, "jo_attention_workspace_bytes": _I64}
 
 # name -> argument types, in header order.
 SIGNATURES: dict[str, list] = {
@@ -92,6 +92,19 @@ SIGNATURES: dict[str, list] = {
     "jo_kv_commit_rope": [
         _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
         _I64, _P, _P, _I64, _I64, c_int, _P],
+    "jo_paged_tables": [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P,
+                        _P, _P],
+    "jo_kv_commit_rope_paged": [
+        _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
+        _P, _I64, c_int, _P],
+    "jo_attention_varlen": [
+        _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+        _I64, _I64, _P, _P, _F, c_int, c_int, c_int, _P, _I64, _P],
+    "jo_attention_paged": [
+        _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+        _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _F, c_int, c_int, c_int, _P, _I64,
+        _P],
+    "jo_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
 }
 
 _lib = None

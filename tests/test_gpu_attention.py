@@ -1,0 +1,412 @@
+"""attention_varlen and attention_paged against the definition in 64 bits, with bounds made of
+the roundings they are allowed (oracle.serving.attention_bound)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import joyomni_ops as jo
+from oracle import serving
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def cu_of(lens):
+    return [0] + torch.tensor(lens, dtype=torch.int64).cumsum(0).tolist() if lens else [0]
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def randn(shape, dtype, seed, mul=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * mul).to(dtype)
+
+
+def seen_mask(n, m, causal, hidden=None):
+    """bool [n, m]: what the i-th of n new tokens sees of m keys; hidden: keys that have no
+    place (bool [m])."""
+    j = torch.arange(m)[None, :]
+    seen = (j <= m - n + torch.arange(n)[:, None]) if causal else torch.ones(n, m, dtype=torch.bool)
+    return seen if hidden is None else seen & ~hidden[None, :]
+
+
+def check(out, q, requests, scale, dtype):
+    """requests: [(q0, q1, k, v, seen)] of the rows that belong to a request."""
+    out = out.cpu()
+    rest = torch.ones(q.shape[0], dtype=torch.bool)
+    for q0, q1, k, v, seen in requests:
+        rest[q0:q1] = False
+        if q1 == q0:
+            continue
+        want, size, score = serving.attention(q[q0:q1], k, v, seen, scale)
+        fin = torch.isfinite(want)
+        got = out[q0:q1].double()
+        v_max = float(v.double().nan_to_num(0, 0, 0).abs().max()) if v.numel() else 0.0
+        bound = serving.attention_bound(dtype, want.nan_to_num(), size.nan_to_num(), score.nan_to_num(),
+                                        int(seen.sum(1).max()) if seen.numel() else 0, v_max)
+        assert bool((torch.isfinite(got) == fin).all()), "finite where the definition is not, or not"
+        err = (got - want).abs()[fin]
+        over = err > bound[fin]
+        assert not bool(over.any()), (
+            f"{int(over.sum())} of {err.numel()} beyond the bound; worst "
+            f"{float((err / bound[fin]).max()):.3f} of it")
+        empty = ~seen.any(1)
+        assert bool((out[q0:q1][empty] == 0).all()), "a row that sees nothing must be zeros"
+    return rest
+
+
+# ---------------------------------------------------------------------------
+# Packed sequences.
+# ---------------------------------------------------------------------------
+def varlen_case(dev, lq, lk, Hq, Hkv, D, dtype, causal, seed=0, pad=0, mul=1.3, packed=False,
+                scale=None, out=None):
+    T, Tk = sum(lq) + pad, sum(lk) + pad
+    if packed:
+        qkv = randn((T, Hq + 2 * Hkv, D), dtype, seed, mul)
+        q, k, v = qkv.split((Hq, Hkv, Hkv), 1)
+        dq = qkv.to(dev)
+        gq, gk, gv = dq.split((Hq, Hkv, Hkv), 1)
+    else:
+        q, k, v = (randn((t, h, D), dtype, seed + i, m)
+                   for i, (t, h, m) in enumerate(((T, Hq, mul), (Tk, Hkv, mul), (Tk, Hkv, 1.0))))
+        gq, gk, gv = q.to(dev), k.to(dev), v.to(dev)
+    cq, ck = cu_of(lq), cu_of(lk)
+    got = jo.attention_varlen(gq, gk, gv, i32(cq, dev), None if lq is lk else i32(ck, dev),
+                              causal=causal, scale=scale, out=out)
+    reqs = [(cq[r], cq[r + 1], k[ck[r]:ck[r + 1]], v[ck[r]:ck[r + 1]],
+             seen_mask(lq[r], lk[r], causal)) for r in range(len(lq))]
+    rest = check(got, q, reqs, scale or D ** -0.5, dtype)
+    if out is None:
+        assert bool((got.cpu()[rest] == 0).all())
+    return got
+
+
+LENS = [[1], [2, 1, 1], [0, 5, 0, 64, 65, 1, 0], [127, 128, 129], [300], [17] * 9, [31, 33, 16, 15],
+        [255, 1, 257]]
+
+
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("dtype", (BF16, FP16))
+def test_varlen_lengths(dev, dtype, lens, causal):
+    varlen_case(dev, lens, lens, 4, 2, 128, dtype, causal)
+
+
+@pytest.mark.parametrize("D", (64, 128, 256))
+@pytest.mark.parametrize("heads", ((1, 1), (3, 3), (6, 2), (5, 1), (7, 1), (16, 1), (20, 1), (40, 2), (8, 8)),
+                         ids=lambda x: f"{x[0]}over{x[1]}")
+def test_varlen_heads(dev, heads, D):
+    lens = [3, 70, 1, 130]
+    varlen_case(dev, lens, lens, *heads, D, BF16, True, seed=1)
+    varlen_case(dev, lens, lens, *heads, D, FP16, False, seed=2)
+
+
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("lq,lk", (([5, 9], [0, 3]), ([1, 1, 1], [500, 0, 1]), ([40], [1700]),
+                                   ([100, 3], [20, 64]), ([0, 7], [9, 7]), ([64, 0], [0, 0]),
+                                   ([200], [64]), ([33], [2100])))
+def test_varlen_cross_lengths(dev, lq, lk, causal):
+    """Fewer keys than tokens leave the first tokens with nothing to see (causal)."""
+    for D in (64, 128, 256):
+        varlen_case(dev, lq, lk, 4, 2, D, BF16, causal, seed=3)
+
+
+@pytest.mark.parametrize("D", (64, 128, 256))
+@pytest.mark.parametrize("heads", ((4, 4), (8, 2)))
+def test_varlen_packed_projection(dev, heads, D):
+    lens = [77, 12, 140]
+    varlen_case(dev, lens, lens, *heads, D, BF16, True, seed=4, packed=True)
+
+
+def test_varlen_scale_and_peaked_scores(dev):
+    lens = [90, 200]
+    varlen_case(dev, lens, lens, 4, 2, 128, BF16, True, seed=5, scale=0.5)
+    varlen_case(dev, lens, lens, 4, 2, 64, FP16, False, seed=6, mul=6.0)
+    varlen_case(dev, lens, lens, 4, 2, 128, BF16, True, seed=7, scale=1e-3)
+
+
+def test_rows_behind_the_last_sequence(dev):
+    lens = [60, 9]
+    varlen_case(dev, lens, lens, 4, 2, 128, BF16, True, seed=8, pad=201)  # zeros in a new tensor
+    out = torch.full((270, 4, 128), 7.0, dtype=BF16, device=dev)
+    got = varlen_case(dev, lens, lens, 4, 2, 128, BF16, True, seed=8, pad=201, out=out)
+    assert got is out
+    assert bool((out[69:] == 7).all())
+
+
+def test_strided_out_keeps_its_gaps(dev):
+    lens = [60, 9, 130]
+    big = torch.full((199, 6, 200), 3.0, dtype=BF16, device=dev)
+    out = big[:, 1:5, 8:136]
+    varlen_case(dev, lens, lens, 4, 2, 128, BF16, True, seed=9, out=out)
+    keep = big.clone()
+    keep[:, 1:5, 8:136] = 3.0
+    assert bool((keep == 3).all())
+
+
+def test_no_requests_and_no_tokens(dev):
+    q = torch.ones(5, 2, 64, dtype=BF16, device=dev)
+    assert bool((jo.attention_varlen(q, q, q, i32([0], dev)) == 0).all())
+    e = q[:0]
+    assert jo.attention_varlen(e, e, e, i32([0, 0], dev)).shape == (0, 2, 64)
+    assert bool((jo.attention_varlen(q, e, e, i32([0, 5], dev), i32([0, 0], dev)) == 0).all())
+
+
+@pytest.mark.parametrize("bad", (math.nan, math.inf, -math.inf))
+@pytest.mark.parametrize("D", (64, 128, 256))
+def test_later_tokens_do_not_reach_earlier_ones(dev, D, bad):
+    """NaN and infinities in k and v of the token at place 100: the tokens before it, and every
+    other sequence, are as if it were not there."""
+    lens, Hq, Hkv = [150, 120, 40], 4, 2
+    cu = cu_of(lens)
+    q, k, v = (randn((sum(lens), h, D), BF16, 10 + i) for i, h in enumerate((Hq, Hkv, Hkv)))
+    clean = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32(cu, dev)).cpu()
+    at = cu[1] + 100
+    v[at, :, ::3] = bad
+    k[at, :, ::5] = math.nan
+    got = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32(cu, dev)).cpu()
+    before = torch.ones(sum(lens), dtype=torch.bool)
+    before[at:cu[2]] = False
+    assert bool(torch.isfinite(got[before]).all())
+    reqs = [(cu[r], cu[r + 1], k[cu[r]:cu[r + 1]], v[cu[r]:cu[r + 1]],
+             seen_mask(lens[r], lens[r], True)) for r in (0, 2)]
+    n = 100
+    reqs.append((cu[1], cu[1] + n, k[cu[1]:cu[1] + n], v[cu[1]:cu[1] + n], seen_mask(n, n, True)))
+    check(got, q, reqs, D ** -0.5, BF16)
+    assert bool(torch.isnan(got[at:cu[2]]).all())  # who sees a NaN score has no result
+    assert bool((clean[:cu[1]] == got[:cu[1]]).all())
+
+
+def test_seen_infinities_are_the_definition_s(dev):
+    """An infinite v that is seen gives infinities in its own columns alone."""
+    lens, D = [70], 128
+    q, k, v = (randn((70, 1, D), BF16, 20 + i) for i in range(3))
+    v[30, 0, 5] = math.inf
+    got = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32([0, 70], dev)).cpu()
+    assert bool(torch.isinf(got[30:, 0, 5]).all()) and bool(torch.isfinite(got[:30]).all())
+    other = torch.arange(D) != 5
+    assert bool(torch.isfinite(got[:, :, other]).all())
+
+
+def test_lengths_outside_the_tensors_are_cut(dev):
+    """cu_q past the tokens: the sequences end with the tensor."""
+    q, k, v = (randn((50, 2, 64), BF16, 30 + i) for i in range(3))
+    got = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32([0, 20, 1000], dev))
+    want = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32([0, 20, 50], dev))
+    assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------
+# Paged keys.
+# ---------------------------------------------------------------------------
+def paged_case(dev, new, ctx, P, Hq, Hkv, D, dtype, causal, seed=0, holes=(), fill=math.nan,
+               head_major=False, extra_width=2, pad=0, scale=None, mul=1.3):
+    """Requests of new[r] tokens over ctx[r] cached ones and their own. Every place of the pool
+    that holds no key of a request is `fill`; holes: (request, column) entries without a page."""
+    R = len(new)
+    keys = [n + c for n, c in zip(new, ctx)]
+    need = [-(-m // P) for m in keys]
+    W, N = max(need + [1]) + extra_width, sum(need) + 3
+    g = torch.Generator().manual_seed(seed)
+    order = torch.randperm(N, generator=g).tolist()
+    q = randn((sum(new) + pad, Hq, D), dtype, seed + 1, mul)
+    shape = (N, Hkv, P, D) if head_major else (N, P, Hkv, D)
+    pk, pv = (torch.full(shape, fill, dtype=dtype) for _ in range(2))
+    vk, vv = (x.transpose(1, 2) if head_major else x for x in (pk, pv))
+    table = torch.full((R, W), -1, dtype=torch.int32)
+    cq, reqs = cu_of(new), []
+    for r in range(R):
+        pages = [order.pop() for _ in range(need[r])]
+        table[r, :need[r]] = torch.tensor(pages, dtype=torch.int32)
+        table[r, need[r]:] = 10 ** 6 if r % 2 else -1  # never looked at
+        k, v = (randn((keys[r], Hkv, D), dtype, seed + 10 * r + 2 + i, m)
+                for i, m in enumerate((mul, 1.0)))
+        hidden = torch.zeros(keys[r], dtype=torch.bool)
+        for j in range(keys[r]):
+            vk[pages[j // P], j % P], vv[pages[j // P], j % P] = k[j], v[j]
+        for hr, col in holes:
+            if hr == r and col < need[r]:
+                table[r, col] = -1 if col % 2 else N + col
+                hidden[col * P:(col + 1) * P] = True
+        reqs.append((cq[r], cq[r + 1], k, v, seen_mask(new[r], keys[r], causal, hidden)))
+    dk, dv = pk.to(dev), pv.to(dev)
+    if head_major:
+        dk, dv = dk.transpose(1, 2), dv.transpose(1, 2)
+    got = jo.attention_paged(q.to(dev), dk, dv, table.to(dev), i32(cq, dev), i32(keys, dev),
+                             causal=causal, scale=scale)
+    rest = check(got, q, reqs, scale or D ** -0.5, dtype)
+    assert bool((got.cpu()[rest] == 0).all())
+    return got
+
+
+@pytest.mark.parametrize("P", (1, 7, 16, 52, 64, 128))
+@pytest.mark.parametrize("D,dtype", ((64, BF16), (128, BF16), (256, BF16), (128, FP16)))
+def test_paged_single_tokens(dev, D, dtype, P):
+    paged_case(dev, [1] * 6, [0, 1, 15, 64, 130, 333], P, 8, 2, D, dtype, True)
+
+
+@pytest.mark.parametrize("P", (1, 16, 52, 64))
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("D", (64, 128, 256))
+def test_paged_chunks(dev, D, causal, P):
+    paged_case(dev, [5, 0, 1, 70, 33, 128], [40, 9, 200, 0, 64, 31], P, 4, 2, D, BF16, causal, seed=1)
+
+
+@pytest.mark.parametrize("heads", ((1, 1), (3, 3), (6, 2), (5, 1), (16, 1), (20, 1), (33, 1), (12, 4)),
+                         ids=lambda x: f"{x[0]}over{x[1]}")
+def test_paged_heads(dev, heads):
+    for D in (64, 128, 256):
+        paged_case(dev, [1, 2, 1, 9], [70, 3, 0, 100], 16, *heads, D, BF16, True, seed=2)
+
+
+@pytest.mark.parametrize("new,ctx", (([1], [5000]), ([1, 1], [4000, 3]), ([3], [3000]), ([70], [2500]),
+                                     ([1] * 40, [37 * i % 900 for i in range(40)]),
+                                     ([1, 200, 1, 1], [2000, 700, 1, 0])))
+@pytest.mark.parametrize("D", (64, 128, 256))
+def test_paged_long_keys_are_split(dev, D, new, ctx):
+    paged_case(dev, new, ctx, 16, 4, 1, D, BF16, True, seed=3)
+    paged_case(dev, new, ctx, 52, 2, 2, D, FP16, False, seed=4)
+
+
+@pytest.mark.parametrize("fill", (math.nan, math.inf, 0.0))
+def test_paged_entries_without_a_page(dev, fill):
+    """Table entries that name no page: their keys are not there, whatever page 0 holds."""
+    holes = ((0, 0), (1, 1), (1, 2), (2, 0), (2, 1), (3, 5))
+    for D in (64, 128):
+        for new in ([1, 1, 1, 1], [40, 3, 70, 20]):
+            paged_case(dev, new, [100, 200, 10, 333], 32, 4, 2, D, BF16, True, seed=5, holes=holes,
+                       fill=fill)
+
+
+def test_paged_head_major_pages(dev):
+    paged_case(dev, [1, 40, 1], [77, 100, 0], 16, 8, 2, 128, BF16, True, seed=6, head_major=True)
+
+
+def test_paged_padded_step(dev):
+    paged_case(dev, [1, 1, 30], [77, 100, 0], 16, 8, 2, 128, BF16, True, seed=7, pad=97)
+
+
+def test_paged_more_new_tokens_than_keys(dev):
+    """kv_lens below a request's tokens: the first ones see nothing."""
+    D, dtype = 128, BF16
+    q, pk, pv = randn((9, 2, D), dtype, 1), randn((2, 4, 2, D), dtype, 2), randn((2, 4, 2, D), dtype, 3)
+    got = jo.attention_paged(q.to(dev), pk.to(dev), pv.to(dev), i32([[1, 0]], dev), i32([0, 9], dev),
+                             i32([5], dev))
+    k, v = (x[[1, 0]].flatten(0, 1)[:5] for x in (pk, pv))
+    check(got, q, [(0, 9, k, v, seen_mask(9, 5, True))], D ** -0.5, dtype)
+
+
+def test_paged_lengths_past_the_table(dev):
+    """kv_lens past what the table's rows can place: keys end with the table, positions do not."""
+    D, dtype = 128, BF16
+    q, pk, pv = randn((1, 2, D), dtype, 1), randn((3, 4, 2, D), dtype, 2), randn((3, 4, 2, D), dtype, 3)
+    got = jo.attention_paged(q.to(dev), pk.to(dev), pv.to(dev), i32([[2, 0]], dev), i32([0, 1], dev),
+                             i32([2 ** 31 - 1], dev))
+    k, v = (x[[2, 0]].flatten(0, 1) for x in (pk, pv))
+    check(got, q, [(0, 1, k, v, torch.ones(1, 8, dtype=torch.bool))], D ** -0.5, dtype)
+    none = jo.attention_paged(q.to(dev), pk[:0].to(dev), pv[:0].to(dev), i32([[2, 0]], dev),
+                              i32([0, 1], dev), i32([4], dev))
+    assert bool((none == 0).all())
+
+
+@pytest.mark.parametrize("new", (1, 40))
+def test_paged_pool_past_32_bits(dev, new):
+    """A pool of 2^31 elements and more (4.3 GB each of K and V): its last pages."""
+    P, Hkv, D, ctx = 64, 8, 128, 300
+    N = 2 ** 31 // (P * Hkv * D) + 9
+    pk, pv = (torch.empty((N, P, Hkv, D), dtype=BF16, device=dev) for _ in range(2))
+    m = ctx + new
+    need = -(-m // P)
+    q, k, v = randn((new, 16, D), BF16, 1), randn((m, Hkv, D), BF16, 2), randn((m, Hkv, D), BF16, 3)
+    pages = [N - 1 - i for i in range(need)]
+    for i, p in enumerate(pages):
+        part = slice(i * P, min(m, (i + 1) * P))
+        n = part.stop - part.start
+        pk[p, :n], pv[p, :n] = k[part].to(dev), v[part].to(dev)
+    got = jo.attention_paged(q.to(dev), pk, pv, i32([pages], dev), i32([0, new], dev), i32([m], dev))
+    check(got, q, [(0, new, k, v, seen_mask(new, m, True))], D ** -0.5, BF16)
+
+
+# ---------------------------------------------------------------------------
+# Streams, graphs, repeats.
+# ---------------------------------------------------------------------------
+def step_inputs(dev, seed=0, new=(1, 1, 40, 1), ctx=(700, 20, 100, 3000), P=16):
+    keys = [n + c for n, c in zip(new, ctx)]
+    need = [-(-m // P) for m in keys]
+    N, W = sum(need), max(need)
+    table = torch.full((len(new), W), -1, dtype=torch.int32)
+    at = 0
+    for r, n in enumerate(need):
+        table[r, :n] = torch.arange(at, at + n)
+        at += n
+    q = randn((sum(new), 8, 128), BF16, seed, 1.3).to(dev)
+    pk, pv = (randn((N, P, 2, 128), BF16, seed + i).to(dev) for i in (1, 2))
+    return q, pk, pv, table.to(dev), i32(cu_of(list(new)), dev), i32(keys, dev)
+
+
+def test_same_call_same_bits(dev):
+    args = step_inputs(dev)
+    first = jo.attention_paged(*args)
+    for _ in range(3):
+        assert torch.equal(jo.attention_paged(*args), first)
+
+
+def test_side_stream(dev):
+    args = step_inputs(dev)
+    want = jo.attention_paged(*args)
+    s = torch.cuda.Stream(dev)
+    s.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(s):
+        got = jo.attention_paged(*args)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_two_captured_graphs_with_new_lengths(dev):
+    """Two graphs of different steps, replayed in turn with eager work between, lengths and
+    inputs changed in place: every replay equals the eager call."""
+    a, b = step_inputs(dev, 1), step_inputs(dev, 2, new=(1, 1, 1, 1), ctx=(5000, 20, 9, 0))
+    graphs, outs = [], []
+    for args in (a, b):
+        jo.attention_paged(*args)
+        torch.cuda.synchronize(dev)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = jo.attention_paged(*args)
+        graphs.append(g)
+        outs.append(o)
+    for k in range(4):
+        for args, g, o in ((a, graphs[0], outs[0]), (b, graphs[1], outs[1])):
+            args[0].copy_(randn(tuple(args[0].shape), BF16, 50 + k, 1.3))
+            args[5].sub_(3 if k % 2 else 0).clamp_(min=0)
+            want = jo.attention_paged(*args)
+            g.replay()
+            torch.cuda.synchronize(dev)
+            assert torch.equal(o, want), k
+
+
+def test_paged_equals_packed(dev):
+    """The same keys in pages and packed: whole prompts through both entry points."""
+    lens, Hq, Hkv, D, P = [130, 7, 64], 8, 2, 128, 16
+    q, k, v = (randn((sum(lens), h, D), BF16, 60 + i).to(dev) for i, h in enumerate((Hq, Hkv, Hkv)))
+    cu = i32(cu_of(lens), dev)
+    packed = jo.attention_varlen(q, k, v, cu)
+    need = [-(-n // P) for n in lens]
+    pk, pv = (torch.zeros(sum(need), P, Hkv, D, dtype=BF16, device=dev) for _ in range(2))
+    table, at = torch.full((3, max(need)), -1, dtype=torch.int32), 0
+    for r, n in enumerate(lens):
+        for j in range(need[r]):
+            rows = slice(cu_of(lens)[r] + j * P, min(cu_of(lens)[r + 1], cu_of(lens)[r] + (j + 1) * P))
+            m = rows.stop - rows.start
+            pk[at, :m], pv[at, :m], table[r, j] = k[rows], v[rows], at
+            at += 1
+    paged = jo.attention_paged(q, pk, pv, table.to(dev), cu, i32(lens, dev))
+    diff = (paged.float() - packed.float()).abs()
+    # Both within their bound of the same value: together twice a step of bf16 of the terms' size.
+    assert float(diff.max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
