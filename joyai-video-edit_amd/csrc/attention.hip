@@ -3,6 +3,8 @@
 // prompts). The formulas and the rules of what a token sees are with
 // jo_attention_varlen in joyomni_hip.h.
 
+#include <type_traits>
+
 #include "jo_device.hpp"
 #include "jo_host.hpp"
 
@@ -28,6 +30,10 @@ struct AttnArgs {
   FastDiv fd_page, fd_group;
   float scale_log2;                  // scale * log2(e): softmax in powers of two
   int32_t causal, fill_rest;
+  uint32_t k_ps16, k_ts16, v_ps16, v_ts16;  // strides in units of 16 bytes
+  uint32_t items;                    // work items launched, a key head each
+  uint32_t split_target;             // 0: keys are not split
+  float* ws;                         // partial results of split items
 };
 
 // A request's share of the packed arrays, with every bound clamped: what the
@@ -60,17 +66,6 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int r) {
 // Keys [0, n) that the i-th query token of the request may see.
 __device__ __forceinline__ int32_t visible(const AttnArgs& a, const Request& x, int32_t i) {
   return a.causal ? max(0, min(x.keys, x.first_pos + i + 1)) : x.keys;
-}
-
-// The last r with cu_q[r] <= t (0 if none): the owner of token t, if it has one.
-__device__ __forceinline__ int find_request(const AttnArgs& a, int32_t t) {
-  int lo = 0, hi = a.requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (a.cu_q[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
 }
 
 // Element offset of key j's row in a page (K's or V's strides), or -1 if its
@@ -150,48 +145,895 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, int r, const Reque
   l_out = l;
 }
 
-template <class Tag, int D, bool PAGED>
-__global__ __launch_bounds__(kBlock) void attn_rows_kernel(const AttnArgs a) {
+// ---------------------------------------------------------------------------
+// Work items. A request's rows are its (token, head of the group) pairs, token
+// first: the query heads that share a key head share its K and V tiles. A tile
+// is ROWS consecutive rows of one request and one key head; where there are few
+// tiles, or requests of very different lengths, a tile's keys are split into
+// ranges of `chunk` key blocks of kKeyBlock, a workgroup each, whose partial
+// results a second kernel joins.
+//
+// No host knows the lengths: a workgroup finds its own item from its index.
+// With up to kPlanRequests requests each wave scans their lengths (four a lane):
+//   cost = sum over requests of tiles x key blocks,
+//   chunk = max(kMinChunk, ceil(cost / split_target)),
+//   splits = ceil(key blocks / chunk), items = tiles x splits, in request order,
+// so there are at most tiles + split_target items, which is what is launched.
+// With more requests keys are not split, and request r's tiles begin at index
+// floor(cu_q[r] x group / ROWS) + r, which leaves each room for its tiles.
+// ---------------------------------------------------------------------------
+constexpr int kKeyBlock = 64;
+constexpr int kPlanPerLane = 4;
+constexpr int kPlanRequests = kPlanPerLane * kWave;
+constexpr int kMinChunk = 4;  // key blocks a split
+constexpr int64_t kMaxKeys = INT32_MAX - 4096;  // room for sums of a key index and a block
+
+struct Item {
+  Request x;
+  int r;               // -1: no work
+  int tile;            // rows [tile * ROWS, ...) of the request
+  int split, splits;   // this range of the keys, and how many there are
+  int chunk;           // key blocks a range
+  int index;           // of the item (a partial result's place); in the joining kernel: of the
+                       // tile's first item
+};
+
+// Inclusive prefix sum over the wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   const int lane = threadIdx.x % kWave;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) +
-                     __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int32_t t = static_cast<int32_t>(id / a.q_heads);
-  const int head = static_cast<int>(id - static_cast<int64_t>(t) * a.q_heads);
-  if (t >= a.q_tokens) return;
-  float o[D / 64] = {}, m, l = 0.f;
-  bool owned = false;
-  if (a.requests > 0) {
-    const int r = find_request(a, t);
-    const Request x = request<PAGED>(a, r);
-    owned = t >= x.q0 && t < x.q0 + x.nq;
-    if (owned)
-      attend_row<Tag, D, PAGED>(a, r, x, head, t - x.q0, 0, visible(a, x, t - x.q0), m, l, o);
-  }
-  if (!owned && !a.fill_rest) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t off = t * a.o_ts + head * a.o_hs;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) store_elem<Tag>(a.out, off + e * 64 + lane, o[e] * inv);
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t up = __shfl_up(v, d);
+    if (lane >= d) v = __builtin_elementwise_add_sat(v, up);
+  }
+  return v;
+}
+
+// The item of index id (TILES: the tile of index id, all its splits).
+template <int ROWS, bool PAGED, bool TILES>
+__device__ __forceinline__ Item find_item(const AttnArgs& a, uint32_t id) {
+  const int lane = threadIdx.x % kWave;
+  Item it;
+  it.r = -1;
+  if (a.requests <= kPlanRequests) {
+    uint32_t tiles[kPlanPerLane], blocks[kPlanPerLane], cost = 0;
+#pragma unroll
+    for (int e = 0; e < kPlanPerLane; ++e) {
+      const int r = lane * kPlanPerLane + e;
+      const Request x = request<PAGED>(a, min(r, a.requests - 1));
+      tiles[e] = r < a.requests ? (static_cast<uint32_t>(x.nq) * a.group + ROWS - 1) / ROWS : 0;
+      blocks[e] = (static_cast<uint32_t>(x.keys) + kKeyBlock - 1) / kKeyBlock;
+      const uint64_t c = static_cast<uint64_t>(tiles[e]) * blocks[e];
+      cost = __builtin_elementwise_add_sat(cost, static_cast<uint32_t>(min(c, uint64_t{UINT32_MAX})));
+    }
+    uint32_t chunk = 0x40000000u;  // beyond any number of key blocks: no split
+    if (a.split_target > 0) {
+      const uint32_t total = __builtin_amdgcn_readlane(wave_scan(cost), kWave - 1);
+      chunk = max(static_cast<uint32_t>(kMinChunk),
+                  total / a.split_target + (total % a.split_target != 0));
+      // A saturated total says too little of the cost: no split.
+      if (total == UINT32_MAX) chunk = 0x40000000u;
+    }
+    uint32_t splits[kPlanPerLane], items = 0, units = 0;
+#pragma unroll
+    for (int e = 0; e < kPlanPerLane; ++e) {
+      splits[e] = max(1u, (blocks[e] + chunk - 1) / chunk);
+      items += tiles[e] * splits[e];
+      units += TILES ? tiles[e] : tiles[e] * splits[e];
+    }
+    const uint32_t unit_end = wave_scan(units);
+    const uint32_t item_end = TILES ? wave_scan(items) : unit_end;
+    const uint64_t past = __ballot(unit_end > id);
+    if (past == 0) return it;
+    const int owner = __builtin_ctzll(past);
+    // In the owner lane: which of its requests, and the index within it.
+    uint32_t local = id - (unit_end - units), first = item_end - items, e_found = 0;
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < kPlanPerLane; ++e) {
+      const uint32_t n = TILES ? tiles[e] : tiles[e] * splits[e];
+      if (!found && local < n) {
+        found = true;
+        e_found = e;
+      }
+      if (!found) {
+        local -= n;
+        first += tiles[e] * splits[e];
+      }
+    }
+    uint32_t n_splits = splits[0], n_tiles = tiles[0];
+#pragma unroll
+    for (int e = 1; e < kPlanPerLane; ++e)
+      if (e_found == e) n_splits = splits[e], n_tiles = tiles[e];
+    local = __builtin_amdgcn_readlane(local, owner);
+    first = __builtin_amdgcn_readlane(first, owner);
+    n_splits = __builtin_amdgcn_readlane(n_splits, owner);
+    n_tiles = __builtin_amdgcn_readlane(n_tiles, owner);
+    it.r = owner * kPlanPerLane + __builtin_amdgcn_readlane(e_found, owner);
+    it.splits = n_splits;
+    it.chunk = chunk;
+    const uint32_t t = TILES ? local : local / n_splits;
+    it.split = TILES ? 0 : local - t * n_splits;
+    // The last tile first: with a causal mask it sees the most keys.
+    it.tile = n_tiles - 1 - t;
+    it.index = TILES ? first + t * n_splits : id;
+    it.x = request<PAGED>(a, it.r);
+    return it;
+  }
+  // 64 ways at a time: the last request whose first index is not above id.
+  int lo = 0, n = a.requests;
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave;
+    const int r = lo + lane * step;
+    bool below = false;
+    if (lane * step < n) {
+      const uint32_t q0 = min(max(a.cu_q[r], 0), a.q_tokens);
+      below = q0 * a.group / ROWS + r <= id;
+    }
+    const uint64_t mask = __ballot(below);
+    const int at = mask == 0 ? 0 : 63 - __builtin_clzll(mask);
+    lo += at * step;
+    n = min(step, n - at * step);
+  }
+  it.x = request<PAGED>(a, lo);
+  const uint32_t rows = static_cast<uint32_t>(it.x.nq) * a.group;
+  const uint32_t begin = static_cast<uint32_t>(it.x.q0) * a.group / ROWS + lo;
+  const uint32_t tiles = (rows + ROWS - 1) / ROWS;
+  if (id < begin || id - begin >= tiles) return it;
+  it.r = lo;
+  it.splits = 1;
+  it.split = 0;
+  it.chunk = 0x40000000;
+  it.index = id;
+  it.tile = tiles - 1 - (id - begin);
+  return it;
+}
+
+// Zeros for the tokens behind the last request, by the workgroups behind the
+// items' (part `part` of `parts`).
+template <class Tag, int D>
+__device__ __forceinline__ void fill_rest(const AttnArgs& a, uint32_t part, uint32_t parts) {
+  const int32_t from = a.requests > 0 ? min(max(a.cu_q[a.requests], 0), a.q_tokens) : 0;
+  constexpr uint32_t C = D / 8;
+  const int64_t pieces = static_cast<int64_t>(a.q_tokens - from) * a.q_heads * C;
+  for (int64_t i = static_cast<int64_t>(part) * blockDim.x + threadIdx.x; i < pieces;
+       i += static_cast<int64_t>(parts) * blockDim.x) {
+    const int64_t row = i / C;
+    const int64_t t = row / a.q_heads, h = row - t * a.q_heads;
+    st16(byte_off(a.out, ((from + t) * a.o_ts + h * a.o_hs + (i - row * C) * 8) * Tag::kBytes),
+         u32x4{0, 0, 0, 0});
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Matrix-core building blocks.
+// ---------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <class Tag>
+__device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (std::is_same<Tag, BF16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <class Tag>
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (std::is_same<Tag, BF16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <class Tag>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<Tag, BF16>::value) return pack_bf16x2(a, b);
+  else return pack_f16x2(a, b);
+}
+
+// An LDS address held in 32 bits, as a pointer.
+#define JO_LDS(type, addr) \
+  ((__attribute__((address_space(3))) type*)(static_cast<uintptr_t>(addr)))
+
+__device__ __forceinline__ u32x4 lds_read16(uint32_t addr) { return *JO_LDS(u32x4, addr); }
+
+// Two transposing reads: within each 16 lanes, lane i names four consecutive
+// elements of row i / 4 and gets column i of the 4 x 16 block: four rows of its
+// own column. Rows here are keys, columns places of head_dim.
+__device__ __forceinline__ u32x4 lds_read_tr(uint32_t addr0, uint32_t addr1) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr0)));
+  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr1)));
+  return u32x4{a.x, a.y, b.x, b.y};
+}
+
+// s_waitcnt limiting only the vector-memory counter to n (n < 64); only the LDS
+// counter to 0.
+#define JO_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(0x0F70 | ((n) & 15) | (((n) >> 4) << 14))
+#define JO_WAIT_LDS0() __builtin_amdgcn_s_waitcnt(0xC07F)
+// Keeps memory accesses on their side of it (the compiler does not know what the
+// waits above wait for).
+#define JO_KEEP_ORDER() asm volatile("" ::: "memory")
+
+// A key row of D elements is D / 8 chunks of 16 bytes; chunk c of row r of a
+// tile in LDS sits at chunk position c ^ swz(r). The 32 banks of 8 bytes hold
+// 16 chunks: K reads take the same chunk of 16 consecutive rows, which swz_k
+// sends to 16 different ones; V's transposing reads take four (32-row tiles) or
+// two (16-row tiles) neighbouring chunks of 8 or 16 consecutive rows, which
+// swz_v32 / swz_k spread evenly.
+template <int D>
+__device__ __forceinline__ constexpr int swz_k(int r) {
+  return D == 64 ? (r >> 1) & 7 : r & 15;
+}
+template <int D>
+__device__ __forceinline__ constexpr int swz_v32(int r) {
+  return D == 64 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+// Where the rows of a block of keys lie: the lane's key (base + lane, cut to
+// the range's last) as offsets of 16 bytes into K and V, and which keys are there.
+struct KeyRows {
+  uint32_t k16, v16;
+  uint64_t there;  // wave-uniform, bit i: key base + i is in the range and has a page
+};
+
+// The first half of key_rows: the page id load, so that it can run ahead.
+template <bool PAGED>
+__device__ __forceinline__ int32_t key_page(const AttnArgs& a, int r, int32_t base, int32_t end) {
+  if constexpr (PAGED) {
+    const int32_t j = min(base + static_cast<int32_t>(threadIdx.x % kWave), end - 1);
+    return a.table[r * a.table_stride + fdiv(j, a.fd_page)];
+  }
+  return 0;
+}
+template <bool PAGED>
+__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Request& x, int32_t page,
+                                            int32_t base, int32_t end) {
+  const int lane = threadIdx.x % kWave;
+  const int32_t j = min(base + lane, end - 1);
+  KeyRows k;
+  bool there = base + lane < end;
+  if constexpr (PAGED) {
+    const uint32_t place = j - fdiv(j, a.fd_page) * a.fd_page.d;
+    const bool has = page >= 0 && page < a.num_pages;
+    there = there && has;
+    const uint32_t p = has ? page : 0;  // keys without a page read page 0: never used
+    k.k16 = p * a.k_ps16 + place * a.k_ts16;
+    k.v16 = p * a.v_ps16 + place * a.v_ts16;
+  } else {
+    k.k16 = static_cast<uint32_t>(x.k0 + j) * a.k_ts16;
+    k.v16 = static_cast<uint32_t>(x.k0 + j) * a.v_ts16;
+  }
+  k.there = __ballot(there);
+  return k;
+}
+
+// Direct global -> LDS loads of ROWS key rows, 16 bytes a lane, written in row
+// order from lds_base on: load i of the COUNT that this wave makes fills rows
+// first_row + i * (rows a load). SRC: the lanes whose offsets these are.
+template <int D, int COUNT, bool V32>
+__device__ __forceinline__ void load_rows(const char* base, uint32_t off16, uint32_t lds_base,
+                                          int first_row, int lane) {
+  constexpr int C = D / 8, PER = kWave / C;  // chunks a row, rows a load
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    const int row = first_row + i * PER + lane / C;
+    const int sw = V32 ? swz_v32<D>(row) : swz_k<D>(row);
+    const uint32_t off = __shfl(off16, row) + ((lane % C) ^ sw);
+    __builtin_amdgcn_global_load_lds(
+        base + (static_cast<uint64_t>(off) << 4),
+        JO_LDS(void, lds_base + static_cast<uint32_t>((first_row + i * PER) * D * 2)), 16, 0, 0);
+  }
+}
+
+// Whether every element of a result row so far is finite (NaN and infinities
+// have all exponent bits set).
+__device__ __forceinline__ bool all_finite(float v) { return finite_bits(v); }
+
+// Rows whose result came out not finite are worked out again, one by one, from
+// the keys they see alone: a tile multiplies every key's v with every row's
+// weight, and the zero weight of a key that a row does not see times a NaN or
+// an infinity is NaN. What is not finite after that is the definition's.
+// `o`, `m`, `l` of the row: lane holds elements e * 64 + lane.
+template <class Tag, int D>
+__device__ __forceinline__ void store_row(const AttnArgs& a, const Item& it, int kv_head, int row,
+                                          int local_row, int rows_per_tile, float m, float l,
+                                          const float (&o)[D / 64]) {
+  const int lane = threadIdx.x % kWave;
+  if (it.splits == 1) {
+    const int i = fdiv(row, a.fd_group);
+    const int head = kv_head * a.group + row - i * a.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t off = (it.x.q0 + i) * a.o_ts + head * a.o_hs;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) store_elem<Tag>(a.out, off + e * 64 + lane, o[e] * inv);
+  } else {
+    float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * rows_per_tile * (D + 2);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) part[local_row * D + e * 64 + lane] = o[e];
+    if (lane == 0) {
+      part[rows_per_tile * D + local_row] = m;
+      part[rows_per_tile * (D + 1) + local_row] = l;
+    }
+  }
+}
+
+// Largest growth of a row's maximum (as a power of two) that is let pass
+// without scaling what is summed so far: the weights then reach 2^8 instead of
+// 1, which costs fp32 sums nothing and keeps 16-bit weights in range.
+constexpr float kLazyMax = 8.f;
+
+// ---------------------------------------------------------------------------
+// Many rows: WAVES waves of 32 rows each over blocks of 64 keys that they share.
+//
+// Scores are taken transposed, S^T = K Q^T with 32x32x16 products: a lane then
+// holds 32 keys' scores of one row (column lane % 32, keys 8 a + 4 (lane / 32)
+// + b), so the softmax is arithmetic within a lane but for one exchange between
+// the wave's halves, and the weights P^T are in place as the second operand of
+// O^T = V^T P^T: a product's 16 key slots may stand for any 16 keys as long as
+// V^T's are the same ones, and the transposing LDS reads give a lane four
+// consecutive keys of one column of V at a time, just those.
+// K and V blocks go straight from global memory to LDS, one block ahead of
+// their use; one barrier a block.
+// ---------------------------------------------------------------------------
+template <class Tag, int D, int WAVES, bool PAGED>
+__global__ __launch_bounds__(WAVES * kWave, D <= 128 ? 2 : 1) void attn_tiles_kernel(
+    const AttnArgs a) {
+  constexpr int ROWS = WAVES * 32;
+  constexpr int BLOCK = kKeyBlock * D * 2;  // bytes of a K or V block
+  constexpr int PER = kWave / (D / 8);      // rows a load
+  constexpr int COUNT = kKeyBlock / PER / WAVES;
+  constexpr int KK = D / 16, DB = D / 32;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * BLOCK];  // K0 K1 V0 V1
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t id = blockIdx.x;
+  const uint32_t work = a.items * a.kv_heads;
+  if (id >= work) {
+    fill_rest<Tag, D>(a, id - work, gridDim.x - work);
+    return;
+  }
+  const uint32_t item_id = id / a.kv_heads;
+  const int kv_head = id - item_id * a.kv_heads;
+  const Item it = find_item<ROWS, PAGED, false>(a, item_id);
+  if (it.r < 0) return;
+  const Request& x = it.x;
+
+  // Rows of the tile; this wave's, cut to the request's last (those are
+  // computed again and not stored).
+  const int rows = x.nq * a.group;
+  const int row0 = it.tile * ROWS;
+  const int half = lane / 32;
+  const int my_row = row0 + wave * 32 + lane % 32;
+  const int my_i = fdiv(min(my_row, rows - 1), a.fd_group);
+  const int my_head = kv_head * a.group + min(my_row, rows - 1) - my_i * a.group;
+  const int my_end = visible(a, x, my_i);
+  const int last_i = fdiv(min(row0 + ROWS, rows) - 1, a.fd_group);
+  // Keys of the tile's range, and of the wave's first row.
+  const int64_t range0 = static_cast<int64_t>(it.split) * it.chunk * kKeyBlock;
+  const int k_end = static_cast<int>(min(static_cast<int64_t>(visible(a, x, last_i)),
+                                         range0 + static_cast<int64_t>(it.chunk) * kKeyBlock));
+  const int k_begin = static_cast<int>(min(range0, static_cast<int64_t>(k_end)));
+  const int first_end = visible(a, x, fdiv(min(row0 + wave * 32, rows - 1), a.fd_group));
+  const int wave_end =
+      row0 + wave * 32 < rows
+          ? min(k_end, visible(a, x, fdiv(min(row0 + wave * 32 + 31, rows - 1), a.fd_group)))
+          : 0;
+
+  u32x4 q[KK];
+  {
+    const char* p = static_cast<const char*>(a.q) +
+                    ((x.q0 + my_i) * a.q_ts + my_head * a.q_hs + half * 8) * Tag::kBytes;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) q[k] = ld16(p + k * 32);
+  }
+
+  f32x16 o[DB] = {};
+  float m = -INFINITY, l = 0.f;
+
+  const char* kp = static_cast<const char*>(a.k) + kv_head * a.k_hs * Tag::kBytes;
+  const char* vp = static_cast<const char*>(a.v) + kv_head * a.v_hs * Tag::kBytes;
+  const int first_row = wave * (kKeyBlock / WAVES);
+  auto load_block = [&](const KeyRows& kr, int buf) {
+    load_rows<D, COUNT, false>(kp, kr.k16, lds + buf * BLOCK, first_row, lane);
+    load_rows<D, COUNT, true>(vp, kr.v16, lds + (2 + buf) * BLOCK, first_row, lane);
+  };
+
+  const uint32_t k_addr = lds + (lane % 32) * (D * 2) + ((half ^ swz_k<D>(lane % 32)) << 4);
+  // Lane's place in V's transposing reads: key 4 half + i / 4 of a 16-key step,
+  // columns 16 (lane / 16 % 2) + 4 (i % 4) of a 32-column block (i = lane % 16).
+  const int vi = lane % 16;
+  const int v_row = half * 4 + vi / 4;
+  const int v_chunk = (lane / 16 % 2) * 2 + (vi % 4) / 2;
+  const uint32_t v_addr = lds + 2 * BLOCK + v_row * (D * 2) + (vi % 2) * 8;
+
+  if (k_begin < k_end) {
+    KeyRows cur = key_rows<PAGED>(a, x, key_page<PAGED>(a, it.r, k_begin, k_end), k_begin, k_end);
+    load_block(cur, 0);
+    int32_t next_page = k_begin + kKeyBlock < k_end
+                            ? key_page<PAGED>(a, it.r, k_begin + kKeyBlock, k_end)
+                            : 0;
+    int buf = 0;
+    for (int base = k_begin; base < k_end; base += kKeyBlock, buf ^= 1) {
+      // This block is in LDS (own loads: the wait; the other waves': the
+      // barrier), and every wave is done with the other buffer.
+      JO_KEEP_ORDER();
+      JO_WAIT_VM(0);
+      JO_WAIT_LDS0();
+      __builtin_amdgcn_s_barrier();
+      JO_KEEP_ORDER();
+      const uint64_t there = cur.there;
+      if (base + kKeyBlock < k_end) {
+        cur = key_rows<PAGED>(a, x, next_page, base + kKeyBlock, k_end);
+        load_block(cur, buf ^ 1);
+        if (base + 2 * kKeyBlock < k_end)
+          next_page = key_page<PAGED>(a, it.r, base + 2 * kKeyBlock, k_end);
+      }
+      if (base >= wave_end) continue;  // the wave's rows see none of these keys
+
+      f32x16 s[2] = {};
+      const uint32_t ka = k_addr + buf * BLOCK;
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[b] = mfma32<Tag>(lds_read16((ka ^ (k << 5)) + b * 32 * D * 2), q[k], s[b]);
+      }
+      if (base + kKeyBlock > first_end || ~there != 0) {  // uniform
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = b * 32 + (e / 4) * 8 + half * 4 + e % 4;
+            if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
+          }
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+      if (__any(top * a.scale_log2 > m + kLazyMax)) {
+        const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2);
+        const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+        m = m_new;
+        l *= fade;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= fade;
+      }
+      const float m_use = m == -INFINITY ? 0.f : m;
+      u32x4 p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          w[e] = exp2_fast(fmaf(s[k / 2][(k % 2) * 8 + e], a.scale_log2, -m_use));
+          l += w[e];
+        }
+        p[k] = u32x4{pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
+                     pack2<Tag>(w[6], w[7])};
+      }
+      const uint32_t va = v_addr + buf * BLOCK;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const uint32_t row = va + k * 16 * D * 2;
+          const int sw0 = swz_v32<D>(v_row), sw1 = swz_v32<D>(v_row + 8);
+          o[d] = mfma32<Tag>(lds_read_tr(row + (((d * 4 + v_chunk) ^ sw0) << 4),
+                                         row + 8 * D * 2 + (((d * 4 + v_chunk) ^ sw1) << 4)),
+                             p[k], o[d]);
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 32);
+
+  bool fine = true;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) fine = fine && all_finite(o[d][e]);
+  fine = fine && all_finite(l);
+  const uint64_t bad = __ballot(!fine && my_row < rows);
+  if (my_row < rows) {
+    if (it.splits == 1) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      char* out = static_cast<char*>(a.out) +
+                  ((x.q0 + my_i) * a.o_ts + my_head * a.o_hs + half * 4) * Tag::kBytes;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          st8(out + (d * 32 + e * 8) * Tag::kBytes,
+              u32x2{pack2<Tag>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                    pack2<Tag>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)});
+    } else {
+      float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
+      const int row = wave * 32 + lane % 32;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(part + row * D + d * 32 + e * 8 + half * 4) =
+              f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+      if (half == 0) {
+        part[ROWS * D + row] = m;
+        part[ROWS * (D + 1) + row] = l;
+      }
+    }
+  }
+  uint32_t again = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
+  while (again != 0) {
+    const int b = __builtin_ctz(again);
+    again &= again - 1;
+    const int row = row0 + wave * 32 + b;
+    const int i = fdiv(row, a.fd_group);
+    float ro[D / 64], rm, rl;
+    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row - i * a.group, i, k_begin,
+                              min(k_end, visible(a, x, i)), rm, rl, ro);
+    store_row<Tag, D>(a, it, kv_head, row, wave * 32 + b, ROWS, rm, rl, ro);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (single tokens): 16 rows a workgroup, its waves sharing the keys, 32
+// at a time each, with 16x16x32 products in the same transposed form. Every
+// wave loads its own keys into its own part of LDS, a block ahead, and waits for
+// no other wave until the waves' results are joined at the end.
+// ---------------------------------------------------------------------------
+template <int D>
+struct FewShape {
+  static constexpr int kWaves = D == 256 ? 2 : 4;
+  static constexpr int kKeys = 32;                 // keys a block
+  static constexpr int kBlockBytes = kKeys * D * 2;  // of K or V
+  static constexpr int kWaveBytes = 4 * kBlockBytes;
+  static constexpr int kRowFloats = D + 4;         // a joined row in LDS
+};
+
+template <class Tag, int D, bool PAGED>
+__global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel(const AttnArgs a) {
+  using S = FewShape<D>;
+  constexpr int ROWS = 16, W = S::kWaves, BLOCK = S::kBlockBytes;
+  constexpr int PER = kWave / (D / 8), COUNT = S::kKeys / PER;
+  constexpr int KK = D / 32, DB = D / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[W * S::kWaveBytes];
+  __shared__ float s_m[W][ROWS], s_l[W][ROWS];
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t id = blockIdx.x;
+  const uint32_t work = a.items * a.kv_heads;
+  if (id >= work) {
+    fill_rest<Tag, D>(a, id - work, gridDim.x - work);
+    return;
+  }
+  const uint32_t item_id = id / a.kv_heads;
+  const int kv_head = id - item_id * a.kv_heads;
+  const Item it = find_item<ROWS, PAGED, false>(a, item_id);
+  if (it.r < 0) return;
+  const Request& x = it.x;
+
+  const int rows = x.nq * a.group;
+  const int row0 = it.tile * ROWS;
+  const int grp = lane / 16;
+  const int my_row = min(row0 + lane % 16, rows - 1);
+  const int my_i = fdiv(my_row, a.fd_group);
+  const int my_head = kv_head * a.group + my_row - my_i * a.group;
+  const int my_end = visible(a, x, my_i);
+  const int last_i = fdiv(min(row0 + ROWS, rows) - 1, a.fd_group);
+  const int64_t range0 = static_cast<int64_t>(it.split) * it.chunk * kKeyBlock;
+  const int k_end = static_cast<int>(min(static_cast<int64_t>(visible(a, x, last_i)),
+                                         range0 + static_cast<int64_t>(it.chunk) * kKeyBlock));
+  const int k_begin = static_cast<int>(min(range0, static_cast<int64_t>(k_end)));
+  const int first_end = visible(a, x, fdiv(row0, a.fd_group));
+
+  u32x4 q[KK];
+  {
+    const char* p = static_cast<const char*>(a.q) +
+                    ((x.q0 + my_i) * a.q_ts + my_head * a.q_hs + grp * 8) * Tag::kBytes;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) q[k] = ld16(p + k * 64);
+  }
+  f32x4 o[DB] = {};
+  float m = -INFINITY, l = 0.f;
+
+  const char* kp = static_cast<const char*>(a.k) + kv_head * a.k_hs * Tag::kBytes;
+  const char* vp = static_cast<const char*>(a.v) + kv_head * a.v_hs * Tag::kBytes;
+  const uint32_t mine = lds + wave * S::kWaveBytes;
+  auto load_block = [&](const KeyRows& kr, int buf) {
+    load_rows<D, COUNT, false>(kp, kr.k16, mine + buf * BLOCK, 0, lane);
+    load_rows<D, COUNT, false>(vp, kr.v16, mine + (2 + buf) * BLOCK, 0, lane);
+  };
+  const int kr_ = lane % 16;
+  const uint32_t k_addr = mine + kr_ * (D * 2) + ((grp ^ swz_k<D>(kr_)) << 4);
+  const int vi = lane % 16;
+  const int v_row = grp * 4 + vi / 4;
+  const int v_chunk = (vi % 4) / 2;
+  const uint32_t v_addr = mine + 2 * BLOCK + v_row * (D * 2) + (vi % 2) * 8;
+
+  constexpr int STEP = W * S::kKeys;  // a wave's blocks are this far apart
+  const int my_begin = k_begin + wave * S::kKeys;
+  auto attend = [&](int base, int buf, uint32_t there) {
+          f32x4 s[2] = {};
+          const uint32_t ka = k_addr + buf * BLOCK;
+    #pragma unroll
+          for (int k = 0; k < KK; ++k)
+    #pragma unroll
+            for (int b = 0; b < 2; ++b)
+              s[b] = mfma16<Tag>(lds_read16((ka ^ (k << 6)) + b * 16 * D * 2), q[k], s[b]);
+          if (base + S::kKeys > first_end || ~there != 0) {
+    #pragma unroll
+            for (int b = 0; b < 2; ++b)
+    #pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int j = b * 16 + grp * 4 + e;
+                if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
+              }
+          }
+          float top = fmaxf(s[0][0], s[1][0]);
+    #pragma unroll
+          for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+          if (__any(top * a.scale_log2 > m + kLazyMax)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float m_new = fmaxf(m, top * a.scale_log2);
+            const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+            m = m_new;
+            l *= fade;
+    #pragma unroll
+            for (int d = 0; d < DB; ++d)
+    #pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][e] *= fade;
+          }
+          const float m_use = m == -INFINITY ? 0.f : m;
+          float w[8];
+    #pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w[e] = exp2_fast(fmaf(s[e / 4][e % 4], a.scale_log2, -m_use));
+            l += w[e];
+          }
+          const u32x4 p = {pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
+                           pack2<Tag>(w[6], w[7])};
+          const uint32_t va = v_addr + buf * BLOCK;
+          const int sw0 = swz_k<D>(v_row), sw1 = swz_k<D>(v_row + 16);
+    #pragma unroll
+          for (int d = 0; d < DB; ++d)
+            o[d] = mfma16<Tag>(lds_read_tr(va + (((d * 2 + v_chunk) ^ sw0) << 4),
+                                           va + 16 * D * 2 + (((d * 2 + v_chunk) ^ sw1) << 4)),
+                               p, o[d]);
+  };
+  if (my_begin < k_end) {
+    // Page ids run two blocks ahead of the loads that they are for: in order with
+    // them, a wait for an id is then never a wait for the block just asked for.
+    // (Past the range they read its last entry again.)
+    auto page_at = [&](int base) { return key_page<PAGED>(a, it.r, min(base, k_end - 1), k_end); };
+    KeyRows cur = key_rows<PAGED>(a, x, page_at(my_begin), my_begin, k_end);
+    int32_t page1 = page_at(min(my_begin, k_end - STEP) + STEP);
+    int32_t page2 = page_at(min(my_begin, k_end - 2 * STEP) + 2 * STEP);
+    load_block(cur, 0);
+    int buf = 0, base = my_begin;
+    for (; base < k_end - STEP; base += STEP, buf ^= 1) {
+      const uint32_t there = static_cast<uint32_t>(cur.there);
+      cur = key_rows<PAGED>(a, x, page1, base + STEP, k_end);
+      page1 = page2;
+      page2 = page_at(min(base, k_end - 3 * STEP) + 3 * STEP);
+      JO_KEEP_ORDER();
+      JO_WAIT_LDS0();  // what was read from the other buffer has arrived
+      JO_KEEP_ORDER();
+      load_block(cur, buf ^ 1);
+      JO_KEEP_ORDER();
+      JO_WAIT_VM(2 * COUNT + (PAGED ? 1 : 0));
+      JO_KEEP_ORDER();
+      attend(base, buf, there);
+    }
+    JO_KEEP_ORDER();
+    JO_WAIT_VM(0);
+    JO_KEEP_ORDER();
+    attend(base, buf, static_cast<uint32_t>(cur.there));
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // The waves' results, joined: each wave leaves its 16 rows in its part of LDS.
+  JO_KEEP_ORDER();
+  JO_WAIT_LDS0();
+  JO_KEEP_ORDER();
+  float* mine_o = reinterpret_cast<float*>(smem + wave * S::kWaveBytes);
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+    *reinterpret_cast<f32x4*>(mine_o + (lane % 16) * S::kRowFloats + d * 16 + grp * 4) = o[d];
+  if (grp == 0) {
+    s_m[wave][lane] = m;
+    s_l[wave][lane] = l;
+  }
+  __syncthreads();
+  constexpr int TPR = W * kWave / ROWS;  // threads a row
+  constexpr int NE = D / TPR / 4;        // pieces of four elements a thread
+  const int row = threadIdx.x / TPR, part_of = threadIdx.x % TPR;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][row]);
+  f32x4 r[NE] = {};
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float mw = s_m[w][row];
+    const float e = mw == -INFINITY ? (mw == top ? 1.f : 0.f) : exp2_fast(mw - top);
+    sum = fmaf(e, s_l[w][row], sum);
+    const float* src = reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + row * S::kRowFloats;
+#pragma unroll
+    for (int n = 0; n < NE; ++n) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + (n * TPR + part_of) * 4);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) r[n][c] = fmaf(e, v[c], r[n][c]);
+    }
+  }
+  bool fine = all_finite(sum);
+#pragma unroll
+  for (int n = 0; n < NE; ++n)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) fine = fine && all_finite(r[n][c]);
+  const bool mine_row = row0 + row < rows;
+  uint64_t bad = __ballot(!fine && mine_row);
+  if (mine_row) {
+    if (it.splits == 1) {
+      const int i = fdiv(row0 + row, a.fd_group);
+      const int head = kv_head * a.group + row0 + row - i * a.group;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      char* out = static_cast<char*>(a.out) + ((x.q0 + i) * a.o_ts + head * a.o_hs) * Tag::kBytes;
+#pragma unroll
+      for (int n = 0; n < NE; ++n)
+        st8(out + (n * TPR + part_of) * 4 * Tag::kBytes,
+            u32x2{pack2<Tag>(r[n][0] * inv, r[n][1] * inv), pack2<Tag>(r[n][2] * inv, r[n][3] * inv)});
+    } else {
+      float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
+#pragma unroll
+      for (int n = 0; n < NE; ++n)
+        *reinterpret_cast<f32x4*>(part + row * D + (n * TPR + part_of) * 4) = r[n];
+      if (part_of == 0) {
+        part[ROWS * D + row] = top;
+        part[ROWS * (D + 1) + row] = sum;
+      }
+    }
+  }
+  while (bad != 0) {
+    const int b = __builtin_ctzll(bad) / TPR;  // the wave's b-th row
+    bad &= ~(((TPR == 64 ? 0 : uint64_t{1} << (TPR % 64)) - 1) << (b * TPR));
+    const int local = wave * (kWave / TPR) + b;
+    const int i = fdiv(row0 + local, a.fd_group);
+    float ro[D / 64], rm, rl;
+    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row0 + local - i * a.group, i, k_begin,
+                              min(k_end, visible(a, x, i)), rm, rl, ro);
+    store_row<Tag, D>(a, it, kv_head, row0 + local, local, ROWS, rm, rl, ro);
+  }
+}
+
+// Joins the partial results of split tiles: a workgroup a tile and key head.
+// out = sum_s e_s o_s / sum_s e_s l_s, e_s = 2^(m_s - max m).
+template <class Tag, int D, int ROWS, bool PAGED>
+__global__ __launch_bounds__(kBlock) void attn_join_kernel(const AttnArgs a) {
+  const uint32_t tile_id = blockIdx.x / a.kv_heads;
+  const int kv_head = blockIdx.x - tile_id * a.kv_heads;
+  const Item it = find_item<ROWS, PAGED, true>(a, tile_id);
+  // (A last item that was not launched: lengths that overlap, nothing to join.)
+  if (it.r < 0 || it.splits == 1 || static_cast<uint32_t>(it.index + it.splits) > a.items) return;
+  const int rows = min(ROWS, it.x.nq * a.group - it.tile * ROWS);
+  const int64_t stride = static_cast<int64_t>(a.kv_heads) * ROWS * (D + 2);
+  const float* first = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
+  constexpr int C = D / 4;  // threads a row
+  for (int at = threadIdx.x; at < rows * C; at += kBlock) {
+    const int row = at / C, c = at % C;
+    float top = -INFINITY;
+    for (int s = 0; s < it.splits; ++s) top = fmaxf(top, first[s * stride + ROWS * D + row]);
+    float sum = 0.f;
+    f32x4 r = {};
+    for (int s = 0; s < it.splits; ++s) {
+      const float* p = first + s * stride;
+      const float ms = p[ROWS * D + row], ls = p[ROWS * (D + 1) + row];
+      if (ms == -INFINITY && ls == 0.f) continue;  // sees none of this range
+      const float e = exp2_fast(ms - top);
+      sum = fmaf(e, ls, sum);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(p + row * D + c * 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int i = fdiv(it.tile * ROWS + row, a.fd_group);
+    const int head = kv_head * a.group + it.tile * ROWS + row - i * a.group;
+    st8(byte_off(a.out, ((it.x.q0 + i) * a.o_ts + head * a.o_hs + c * 4) * Tag::kBytes),
+        u32x2{pack2<Tag>(r[0] * inv, r[1] * inv), pack2<Tag>(r[2] * inv, r[3] * inv)});
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launch plan, from sizes that the host has.
+// ---------------------------------------------------------------------------
+struct AttnPlan {
+  bool few;             // attn_few_kernel
+  int64_t tiles;        // at most so many
+  int64_t split_target;
+  int64_t items;
+  int64_t ws_bytes;
+};
+
+constexpr int kTileWaves = 4;
+
+AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                        int64_t head_dim, int64_t kv_capacity) {
+  AttnPlan p;
+  const int64_t group = q_heads / kv_heads;
+  const int64_t all_rows = q_tokens * group;
+  p.few = all_rows <= 16 * requests;
+  const int64_t rows = p.few ? 16 : 32 * kTileWaves;
+  p.tiles = all_rows / rows + (requests < q_tokens || requests > kPlanRequests ? requests : q_tokens);
+  if (requests == 0) p.tiles = 0;
+  const int64_t blocks = (kv_capacity + kKeyBlock - 1) / kKeyBlock;
+  const int64_t groups = p.tiles * kv_heads;
+  p.split_target = 0;
+  if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && groups < 1024)
+    p.split_target = (1024 + kv_heads - 1) / kv_heads;
+  const int64_t most = p.tiles * (blocks / kMinChunk + 1);
+  p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;
+  p.ws_bytes = p.split_target == 0 ? 0 : p.items * kv_heads * rows * (head_dim + 2) * 4;
+  return p;
 }
 
 template <class Tag, int D, bool PAGED>
-int launch_attention(const AttnArgs& a, hipStream_t stream) {
-  const int64_t waves = static_cast<int64_t>(a.q_tokens) * a.q_heads;
-  hipLaunchKernelGGL((attn_rows_kernel<Tag, D, PAGED>), dim3(static_cast<unsigned>((waves + 3) / 4)),
-                     dim3(kBlock), 0, stream, a);
-  return launch_status(PAGED ? "attention_paged" : "attention_varlen");
+int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes,
+                     hipStream_t stream) {
+  const char* op = PAGED ? "attention_paged" : "attention_varlen";
+  AttnPlan p = plan_attention(a.q_tokens, a.requests, a.q_heads, a.kv_heads, D, kv_capacity);
+  if (p.ws_bytes > 0 && ws_bytes < p.ws_bytes) {  // none, or one for another call: no splits
+    p.split_target = 0;
+    p.items = p.tiles;
+  }
+  a.split_target = static_cast<uint32_t>(p.split_target);
+  a.items = static_cast<uint32_t>(p.items);
+  a.ws = static_cast<float*>(ws);
+  // Workgroups that clear the rows of no request, 64 KB each if they are all.
+  const int64_t bytes = static_cast<int64_t>(a.q_tokens) * a.q_heads * D * 2;
+  const int64_t fill = a.fill_rest ? (bytes / 65536 < 256 ? bytes / 65536 + 1 : 256) : 0;
+  const int64_t groups = p.items * a.kv_heads + fill;
+  JO_REQUIRE(groups <= INT32_MAX / 512, "%s: shape too large", op);
+  if (groups == 0) return JO_OK;
+  const dim3 grid(static_cast<unsigned>(groups));
+  if (p.few)
+    hipLaunchKernelGGL((attn_few_kernel<Tag, D, PAGED>), grid, dim3(FewShape<D>::kWaves * kWave), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, kTileWaves, PAGED>), grid,
+                       dim3(kTileWaves * kWave), 0, stream, a);
+  int st = launch_status(op);
+  if (st != JO_OK || p.split_target == 0) return st;
+  const dim3 join(static_cast<unsigned>(p.tiles * a.kv_heads));
+  if (p.few)
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED>), join, dim3(kBlock), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 32 * kTileWaves, PAGED>), join, dim3(kBlock), 0,
+                       stream, a);
+  return launch_status(op);
 }
 
 template <bool PAGED>
-int dispatch_attention(const AttnArgs& a, int64_t head_dim, int dtype, hipStream_t stream) {
+int dispatch_attention(const AttnArgs& a, int64_t head_dim, int dtype, int64_t capacity, void* ws,
+                       int64_t ws_bytes, hipStream_t s) {
   if (dtype == JO_DTYPE_BF16) {
-    if (head_dim == 64) return launch_attention<BF16, 64, PAGED>(a, stream);
-    if (head_dim == 128) return launch_attention<BF16, 128, PAGED>(a, stream);
-    return launch_attention<BF16, 256, PAGED>(a, stream);
+    if (head_dim == 64) return launch_attention<BF16, 64, PAGED>(a, capacity, ws, ws_bytes, s);
+    if (head_dim == 128) return launch_attention<BF16, 128, PAGED>(a, capacity, ws, ws_bytes, s);
+    return launch_attention<BF16, 256, PAGED>(a, capacity, ws, ws_bytes, s);
   }
-  if (head_dim == 64) return launch_attention<F16, 64, PAGED>(a, stream);
-  if (head_dim == 128) return launch_attention<F16, 128, PAGED>(a, stream);
-  return launch_attention<F16, 256, PAGED>(a, stream);
+  if (head_dim == 64) return launch_attention<F16, 64, PAGED>(a, capacity, ws, ws_bytes, s);
+  if (head_dim == 128) return launch_attention<F16, 128, PAGED>(a, capacity, ws, ws_bytes, s);
+  return launch_attention<F16, 256, PAGED>(a, capacity, ws, ws_bytes, s);
 }
 
 // The arguments that both entry points share. Sets q/out/heads/scale fields of `a`.
@@ -235,6 +1077,24 @@ int check_attention(const char* op, AttnArgs& a, const void* q, const void* k, c
   return JO_OK;
 }
 
+// Strides of K and V in units of 16 bytes; row offsets are kept in 32 bits of
+// them (64 GiB from a tensor's start). rows / pages: the largest index + 1.
+int key_offsets(const char* op, AttnArgs& a, int64_t pages, int64_t rows) {
+  auto reach = [](int64_t n, int64_t stride) {  // (n - 1) * stride, 2^40 at most
+    return n <= 1 || stride == 0 ? 0
+           : n - 1 > (int64_t{1} << 40) / stride ? int64_t{1} << 40
+                                                 : (n - 1) * stride;
+  };
+  for (int i = 0; i < 2; ++i) {
+    const int64_t ps = i ? a.v_ps : a.k_ps, ts = i ? a.v_ts : a.k_ts;
+    JO_REQUIRE((reach(pages, ps) + reach(rows, ts)) / 8 <= INT32_MAX * int64_t{2},
+               "%s: K and V rows must lie within 64 GiB", op);
+    (i ? a.v_ps16 : a.k_ps16) = static_cast<uint32_t>(pages > 1 ? ps / 8 : 0);
+    (i ? a.v_ts16 : a.k_ts16) = static_cast<uint32_t>(rows > 1 ? ts / 8 : 0);
+  }
+  return JO_OK;
+}
+
 }  // namespace
 }  // namespace jo
 
@@ -256,7 +1116,7 @@ extern "C" int jo_attention_varlen(const void* q, const void* k, const void* v, 
   a.k_ts = k_token_stride, a.k_hs = k_head_stride;
   a.v_ts = v_token_stride, a.v_hs = v_head_stride;
   a.o_ts = out_token_stride, a.o_hs = out_head_stride;
-  JO_REQUIRE(kv_tokens >= 0 && kv_tokens <= INT32_MAX, "%s: bad shape", op);
+  JO_REQUIRE(kv_tokens >= 0 && kv_tokens <= kMaxKeys, "%s: bad shape", op);
   const int st = check_attention(op, a, q, k, v, out, q_tokens, requests, q_heads, kv_heads,
                                  head_dim, cu_q, scale, dtype);
   if (st != JO_OK || q_tokens == 0) return st;
@@ -265,7 +1125,10 @@ extern "C" int jo_attention_varlen(const void* q, const void* k, const void* v, 
   a.kv_tokens = static_cast<int32_t>(kv_tokens);
   a.causal = causal != 0;
   a.fill_rest = fill_rest != 0;
-  return dispatch_attention<false>(a, head_dim, dtype, static_cast<hipStream_t>(stream));
+  if (const int bad = key_offsets(op, a, 1, kv_tokens); bad != JO_OK) return bad;
+  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16), "%s: workspace must be 16-byte aligned", op);
+  return dispatch_attention<false>(a, head_dim, dtype, kv_tokens, workspace,
+                                   workspace ? workspace_bytes : 0, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int jo_attention_paged(const void* q, const void* pages_k, const void* pages_v,
@@ -303,14 +1166,20 @@ extern "C" int jo_attention_paged(const void* q, const void* pages_k, const void
   // No pages or no table: no key has a place.
   const int64_t places = num_pages == 0 ? 0 : table_width * page_size;
   JO_REQUIRE(places == 0 || (block_table && pages_k && pages_v), "%s: null pointer", op);
-  a.capacity = static_cast<int32_t>(places > INT32_MAX ? INT32_MAX : places);
+  a.capacity = static_cast<int32_t>(places > kMaxKeys ? kMaxKeys : places);
   a.causal = causal != 0;
   a.fill_rest = fill_rest != 0;
-  return dispatch_attention<true>(a, head_dim, dtype, static_cast<hipStream_t>(stream));
+  if (const int bad = key_offsets(op, a, num_pages, page_size); bad != JO_OK) return bad;
+  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16), "%s: workspace must be 16-byte aligned", op);
+  return dispatch_attention<true>(a, head_dim, dtype, table_width * page_size, workspace,
+                                  workspace ? workspace_bytes : 0, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests,
                                                 int64_t q_heads, int64_t kv_heads,
                                                 int64_t head_dim, int64_t kv_capacity) {
-  return 0;
+  if (q_tokens <= 0 || requests < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
+      head_dim <= 0 || kv_capacity < 0)
+    return 0;
+  return plan_attention(q_tokens, requests, q_heads, kv_heads, head_dim, kv_capacity).ws_bytes;
 }
