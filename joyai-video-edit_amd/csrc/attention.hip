@@ -33,8 +33,14 @@ struct AttnArgs {
   uint32_t k_ps16, k_ts16, v_ps16, v_ts16;  // strides in units of 16 bytes
   uint32_t items;                    // work items launched, a key head each
   uint32_t split_target;             // 0: keys are not split
+  FastDiv fd_target;                 // its division
   float* ws;                         // partial results of split items
 };
+
+// Where keys are: packed one behind the other; in pages of a multiple of 16
+// keys (the 16 rows of keys 16 i .. 16 i + 15 are then evenly apart, and one
+// address serves them); in pages of any other size.
+enum class Keys { kPacked, kPages16, kPages };
 
 // A request's share of the packed arrays, with every bound clamped: what the
 // length arrays hold is not trusted to lie inside the tensors.
@@ -44,19 +50,27 @@ struct Request {
   int32_t first_pos;  // position of the first query token: sees keys <= it (causal)
 };
 
+struct RawRequest {
+  int32_t q0, q1, k0, k1;  // k1: paged, the number of keys
+};
 template <bool PAGED>
-__device__ __forceinline__ Request request(const AttnArgs& a, int r) {
+__device__ __forceinline__ RawRequest raw_request(const AttnArgs& a, int r) {
+  return RawRequest{a.cu_q[r], a.cu_q[r + 1], PAGED ? 0 : a.cu_k[r],
+                    PAGED ? a.kv_lens[r] : a.cu_k[r + 1]};
+}
+template <bool PAGED>
+__device__ __forceinline__ Request request(const AttnArgs& a, const RawRequest& w) {
   Request x;
-  x.q0 = min(max(a.cu_q[r], 0), a.q_tokens);
-  x.nq = min(max(a.cu_q[r + 1], x.q0), a.q_tokens) - x.q0;
+  x.q0 = min(max(w.q0, 0), a.q_tokens);
+  x.nq = min(max(w.q1, x.q0), a.q_tokens) - x.q0;
   int32_t len;
   if constexpr (PAGED) {
-    len = max(a.kv_lens[r], 0);
+    len = max(w.k1, 0);
     x.k0 = 0;
     x.keys = min(len, a.capacity);
   } else {
-    x.k0 = min(max(a.cu_k[r], 0), a.kv_tokens);
-    len = min(max(a.cu_k[r + 1], x.k0), a.kv_tokens) - x.k0;
+    x.k0 = min(max(w.k0, 0), a.kv_tokens);
+    len = min(max(w.k1, x.k0), a.kv_tokens) - x.k0;
     x.keys = len;
   }
   x.first_pos = len - x.nq;
@@ -156,13 +170,14 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, int r, const Reque
 // No host knows the lengths: a workgroup finds its own item from its index.
 // With up to kPlanRequests requests each wave scans their lengths (four a lane):
 //   cost = sum over requests of tiles x key blocks,
-//   chunk = max(kMinChunk, ceil(cost / split_target)),
+//   chunk = max(kMinChunk, floor(cost / split_target) + 1),
 //   splits = ceil(key blocks / chunk), items = tiles x splits, in request order,
 // so there are at most tiles + split_target items, which is what is launched.
 // With more requests keys are not split, and request r's tiles begin at index
 // floor(cu_q[r] x group / ROWS) + r, which leaves each room for its tiles.
 // ---------------------------------------------------------------------------
 constexpr int kKeyBlock = 64;
+constexpr int kTileRows = 128;  // of attn_tiles_kernel
 constexpr int kPlanPerLane = 4;
 constexpr int kPlanRequests = kPlanPerLane * kWave;
 constexpr int kMinChunk = 4;  // key blocks a split
@@ -178,88 +193,113 @@ struct Item {
                        // tile's first item
 };
 
-// Inclusive prefix sum over the wave.
+// Inclusive prefix sum over the wave (saturating), with DPP: shifts within rows
+// of 16 lanes, then the rows' totals handed on.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  const int lane = threadIdx.x % kWave;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint32_t up = __shfl_up(v, d);
-    if (lane >= d) v = __builtin_elementwise_add_sat(v, up);
-  }
+#define JO_SCAN_STEP(ctrl, rows) \
+  v = __builtin_elementwise_add_sat( \
+      v, static_cast<uint32_t>( \
+             __builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xf, false)))
+  JO_SCAN_STEP(0x111, 0xf);  // row_shr:1
+  JO_SCAN_STEP(0x112, 0xf);  // row_shr:2
+  JO_SCAN_STEP(0x114, 0xf);  // row_shr:4
+  JO_SCAN_STEP(0x118, 0xf);  // row_shr:8
+  JO_SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+  JO_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef JO_SCAN_STEP
   return v;
 }
 
-// The item of index id (TILES: the tile of index id, all its splits).
-template <int ROWS, bool PAGED, bool TILES>
-__device__ __forceinline__ Item find_item(const AttnArgs& a, uint32_t id) {
+constexpr uint32_t kNoSplit = 0x40000000u;  // beyond any number of key blocks
+
+// find_item with E requests a lane.
+template <int ROWS, bool PAGED, bool TILES, int E>
+__device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
   const int lane = threadIdx.x % kWave;
   Item it;
   it.r = -1;
-  if (a.requests <= kPlanRequests) {
-    uint32_t tiles[kPlanPerLane], blocks[kPlanPerLane], cost = 0;
+  RawRequest raw[E];
 #pragma unroll
-    for (int e = 0; e < kPlanPerLane; ++e) {
-      const int r = lane * kPlanPerLane + e;
-      const Request x = request<PAGED>(a, min(r, a.requests - 1));
-      tiles[e] = r < a.requests ? (static_cast<uint32_t>(x.nq) * a.group + ROWS - 1) / ROWS : 0;
-      blocks[e] = (static_cast<uint32_t>(x.keys) + kKeyBlock - 1) / kKeyBlock;
-      const uint64_t c = static_cast<uint64_t>(tiles[e]) * blocks[e];
-      cost = __builtin_elementwise_add_sat(cost, static_cast<uint32_t>(min(c, uint64_t{UINT32_MAX})));
-    }
-    uint32_t chunk = 0x40000000u;  // beyond any number of key blocks: no split
-    if (a.split_target > 0) {
-      const uint32_t total = __builtin_amdgcn_readlane(wave_scan(cost), kWave - 1);
-      chunk = max(static_cast<uint32_t>(kMinChunk),
-                  total / a.split_target + (total % a.split_target != 0));
-      // A saturated total says too little of the cost: no split.
-      if (total == UINT32_MAX) chunk = 0x40000000u;
-    }
-    uint32_t splits[kPlanPerLane], items = 0, units = 0;
+  for (int e = 0; e < E; ++e) raw[e] = raw_request<PAGED>(a, min(lane * E + e, a.requests - 1));
+  Request x[E];
+  uint32_t tiles[E], blocks[E], cost = 0;
 #pragma unroll
-    for (int e = 0; e < kPlanPerLane; ++e) {
-      splits[e] = max(1u, (blocks[e] + chunk - 1) / chunk);
-      items += tiles[e] * splits[e];
-      units += TILES ? tiles[e] : tiles[e] * splits[e];
-    }
-    const uint32_t unit_end = wave_scan(units);
-    const uint32_t item_end = TILES ? wave_scan(items) : unit_end;
-    const uint64_t past = __ballot(unit_end > id);
-    if (past == 0) return it;
-    const int owner = __builtin_ctzll(past);
-    // In the owner lane: which of its requests, and the index within it.
-    uint32_t local = id - (unit_end - units), first = item_end - items, e_found = 0;
-    bool found = false;
-#pragma unroll
-    for (int e = 0; e < kPlanPerLane; ++e) {
-      const uint32_t n = TILES ? tiles[e] : tiles[e] * splits[e];
-      if (!found && local < n) {
-        found = true;
-        e_found = e;
-      }
-      if (!found) {
-        local -= n;
-        first += tiles[e] * splits[e];
-      }
-    }
-    uint32_t n_splits = splits[0], n_tiles = tiles[0];
-#pragma unroll
-    for (int e = 1; e < kPlanPerLane; ++e)
-      if (e_found == e) n_splits = splits[e], n_tiles = tiles[e];
-    local = __builtin_amdgcn_readlane(local, owner);
-    first = __builtin_amdgcn_readlane(first, owner);
-    n_splits = __builtin_amdgcn_readlane(n_splits, owner);
-    n_tiles = __builtin_amdgcn_readlane(n_tiles, owner);
-    it.r = owner * kPlanPerLane + __builtin_amdgcn_readlane(e_found, owner);
-    it.splits = n_splits;
-    it.chunk = chunk;
-    const uint32_t t = TILES ? local : local / n_splits;
-    it.split = TILES ? 0 : local - t * n_splits;
-    // The last tile first: with a causal mask it sees the most keys.
-    it.tile = n_tiles - 1 - t;
-    it.index = TILES ? first + t * n_splits : id;
-    it.x = request<PAGED>(a, it.r);
-    return it;
+  for (int e = 0; e < E; ++e) {
+    x[e] = request<PAGED>(a, raw[e]);
+    tiles[e] = (static_cast<uint32_t>(x[e].nq) * a.group + ROWS - 1) / ROWS;
+    if (lane * E + e >= a.requests) tiles[e] = 0;
+    blocks[e] = (static_cast<uint32_t>(x[e].keys) + kKeyBlock - 1) / kKeyBlock;
+    const uint64_t c = static_cast<uint64_t>(tiles[e]) * blocks[e];
+    cost = __builtin_elementwise_add_sat(cost, static_cast<uint32_t>(min(c, uint64_t{UINT32_MAX})));
   }
+  uint32_t chunk = kNoSplit;
+  if (a.split_target > 0) {
+    const uint32_t total = __builtin_amdgcn_readlane(wave_scan(cost), kWave - 1);
+    chunk = max(static_cast<uint32_t>(kMinChunk), fdiv(total, a.fd_target) + 1);
+    if (total == UINT32_MAX) chunk = kNoSplit;  // a saturated total says too little
+  }
+  uint32_t splits[E], items = 0, units = 0;
+  // (One division of 32 bits a request; in fp32 first, blocks and chunk being
+  // below 2^24 in any pool that exists, would not hold for all inputs.)
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    splits[e] = blocks[e] <= chunk ? 1u : (blocks[e] - 1) / chunk + 1;
+    items += tiles[e] * splits[e];
+    units += TILES ? (splits[e] > 1 ? tiles[e] : 0) : tiles[e] * splits[e];
+  }
+  const uint32_t unit_end = wave_scan(units);
+  const uint32_t item_end = TILES ? wave_scan(items) : unit_end;
+  const uint64_t past = __ballot(unit_end > id);
+  if (past == 0) return it;
+  const int owner = __builtin_ctzll(past);
+  // In the owner lane: which of its requests, and the index within it.
+  uint32_t local = id - (unit_end - units), first = item_end - items;
+  uint32_t e_found = 0, n_splits = splits[0], n_tiles = tiles[0], n_blocks = blocks[0];
+  Request y = x[0];
+  auto units_of = [&](int e) {
+    return TILES ? (splits[e] > 1 ? tiles[e] : 0) : tiles[e] * splits[e];
+  };
+  bool found = local < units_of(0);
+#pragma unroll
+  for (int e = 1; e < E; ++e) {
+    if (!found) {
+      local -= units_of(e - 1);
+      first += tiles[e - 1] * splits[e - 1];
+      e_found = e, n_splits = splits[e], n_tiles = tiles[e], n_blocks = blocks[e];
+      y = x[e];
+      found = local < units_of(e);
+    }
+  }
+  auto of_owner = [&](auto v) {
+    return static_cast<decltype(v)>(__builtin_amdgcn_readlane(static_cast<int>(v), owner));
+  };
+  local = of_owner(local);
+  first = of_owner(first);
+  n_splits = of_owner(n_splits);
+  n_tiles = of_owner(n_tiles);
+  n_blocks = of_owner(n_blocks);
+  it.x = Request{of_owner(y.q0), of_owner(y.nq), of_owner(y.k0), of_owner(y.keys),
+                 of_owner(y.first_pos)};
+  it.r = owner * E + of_owner(e_found);
+  it.splits = n_splits;
+  // The ranges of a request are of one length, to a block.
+  it.chunk = n_splits == 1 ? kNoSplit : (n_blocks - 1) / n_splits + 1;
+  const uint32_t t = TILES || n_splits == 1 ? local : local / n_splits;
+  it.split = TILES ? 0 : local - t * n_splits;
+  // The last tile first: with a causal mask it sees the most keys.
+  it.tile = n_tiles - 1 - t;
+  it.index = TILES ? first + t * n_splits : id;
+  return it;
+}
+
+// The item of index id (TILES: the split tile of index id, all its splits).
+template <int ROWS, bool PAGED, bool TILES>
+__device__ __forceinline__ Item find_item(const AttnArgs& a, uint32_t id) {
+  if (a.requests <= kWave) return plan_item<ROWS, PAGED, TILES, 1>(a, id);
+  if (a.requests <= kPlanRequests) return plan_item<ROWS, PAGED, TILES, kPlanPerLane>(a, id);
+  const int lane = threadIdx.x % kWave;
+  Item it;
+  it.r = -1;
   // 64 ways at a time: the last request whose first index is not above id.
   int lo = 0, n = a.requests;
   while (n > 1) {
@@ -275,7 +315,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, uint32_t id) {
     lo += at * step;
     n = min(step, n - at * step);
   }
-  it.x = request<PAGED>(a, lo);
+  it.x = request<PAGED>(a, raw_request<PAGED>(a, lo));
   const uint32_t rows = static_cast<uint32_t>(it.x.nq) * a.group;
   const uint32_t begin = static_cast<uint32_t>(it.x.q0) * a.group / ROWS + lo;
   const uint32_t tiles = (rows + ROWS - 1) / ROWS;
@@ -283,7 +323,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& a, uint32_t id) {
   it.r = lo;
   it.splits = 1;
   it.split = 0;
-  it.chunk = 0x40000000;
+  it.chunk = kNoSplit;
   it.index = id;
   it.tile = tiles - 1 - (id - begin);
   return it;
@@ -358,9 +398,12 @@ __device__ __forceinline__ u32x4 lds_read_tr(uint32_t addr0, uint32_t addr1) {
 // counter to 0.
 #define JO_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(0x0F70 | ((n) & 15) | (((n) >> 4) << 14))
 #define JO_WAIT_LDS0() __builtin_amdgcn_s_waitcnt(0xC07F)
+// A lambda that is never a call: what it captures stays in registers.
+#define JO_INLINE __attribute__((always_inline))
 // Keeps memory accesses on their side of it (the compiler does not know what the
 // waits above wait for).
 #define JO_KEEP_ORDER() asm volatile("" ::: "memory")
+
 
 // A key row of D elements is D / 8 chunks of 16 bytes; chunk c of row r of a
 // tile in LDS sits at chunk position c ^ swz(r). The 32 banks of 8 bytes hold
@@ -415,6 +458,35 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Request& x,
   return k;
 }
 
+// 16 bytes a lane from global memory to LDS at the wave-uniform address `lds` on
+// (lane i's at lds + 16 i). In assembly because the compiler, which cannot tell
+// the two LDS buffers apart, would wait for the block being loaded before the
+// transposing reads of the other one; the waits are where the blocks are used.
+// (Of its own loads it then knows too few to be behind them, and waits longer
+// than it must, never shorter.)
+__device__ __forceinline__ void load_to_lds(const char* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
+// A wave-uniform address in scalar registers.
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The same from a wave-uniform address and a 32-bit offset a lane.
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(uniform(base)), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
 // Direct global -> LDS loads of ROWS key rows, 16 bytes a lane, written in row
 // order from lds_base on: load i of the COUNT that this wave makes fills rows
 // first_row + i * (rows a load). SRC: the lanes whose offsets these are.
@@ -427,15 +499,10 @@ __device__ __forceinline__ void load_rows(const char* base, uint32_t off16, uint
     const int row = first_row + i * PER + lane / C;
     const int sw = V32 ? swz_v32<D>(row) : swz_k<D>(row);
     const uint32_t off = __shfl(off16, row) + ((lane % C) ^ sw);
-    __builtin_amdgcn_global_load_lds(
-        base + (static_cast<uint64_t>(off) << 4),
-        JO_LDS(void, lds_base + static_cast<uint32_t>((first_row + i * PER) * D * 2)), 16, 0, 0);
+    load_to_lds(base + (static_cast<uint64_t>(off) << 4),
+                lds_base + static_cast<uint32_t>((first_row + i * PER) * D * 2));
   }
 }
-
-// Whether every element of a result row so far is finite (NaN and infinities
-// have all exponent bits set).
-__device__ __forceinline__ bool all_finite(float v) { return finite_bits(v); }
 
 // Rows whose result came out not finite are worked out again, one by one, from
 // the keys they see alone: a tile multiplies every key's v with every row's
@@ -465,13 +532,92 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const Item& it, int
   }
 }
 
+// max(a, b) that is NaN if either is (v_maximum3_f32, three values an
+// instruction; fmaxf would first make a quiet copy of each).
+__device__ __forceinline__ float nan_max(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
 // Largest growth of a row's maximum (as a power of two) that is let pass
 // without scaling what is summed so far: the weights then reach 2^8 instead of
 // 1, which costs fp32 sums nothing and keeps 16-bit weights in range.
 constexpr float kLazyMax = 8.f;
 
+// The kernel's arguments, read again: what only a kernel's end needs of them is
+// not held in scalar registers (and spilled) through its loop.
+__device__ __forceinline__ AttnArgs args_again() {
+#ifdef __HIP_DEVICE_COMPILE__
+  auto p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const __attribute__((address_space(4))) AttnArgs*)(p);
+#else
+  return AttnArgs{};  // the host's pass over device code
+#endif
+}
+
+// The end of attn_tiles_kernel: 32 rows from row `first` of the tile on, O^T in o
+// (lane: row lane % 32; head_dim 32 d + 8 (e / 4) + 4 (lane / 32) + e % 4), to the
+// output or, of a split tile, to the workspace.
+template <class Tag, int D, int ROWS, bool PAGED>
+__device__ __forceinline__ void store_tile(const AttnArgs a, const Item& it, int kv_head, int first,
+                                           int k_begin, int k_end, const f32x16 (&o)[D / 32],
+                                           float m, float l) {
+  constexpr int DB = D / 32;
+  const Request& x = it.x;
+  const int lane = threadIdx.x % kWave, half = lane / 32;
+  const int rows = x.nq * a.group;
+  const int row0 = it.tile * ROWS;
+  const int my_row = row0 + first + lane % 32;
+  bool fine = finite_bits(l);
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) fine = fine && finite_bits(o[d][e]);
+  const uint64_t bad = __ballot(!fine && my_row < rows);
+  if (my_row < rows) {
+    if (it.splits == 1) {
+      const int i = fdiv(my_row, a.fd_group);
+      const int head = kv_head * a.group + my_row - i * a.group;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      char* out = static_cast<char*>(a.out) +
+                  ((x.q0 + i) * a.o_ts + head * a.o_hs + half * 4) * Tag::kBytes;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          st8(out + (d * 32 + e * 8) * Tag::kBytes,
+              u32x2{pack2<Tag>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                    pack2<Tag>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)});
+    } else {
+      float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
+      const int row = first + lane % 32;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(part + row * D + d * 32 + e * 8 + half * 4) =
+              f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+      if (half == 0) {
+        part[ROWS * D + row] = m;
+        part[ROWS * (D + 1) + row] = l;
+      }
+    }
+  }
+  uint32_t again = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
+  while (again != 0) {
+    const int b = __builtin_ctz(again);
+    again &= again - 1;
+    const int row = row0 + first + b;
+    const int i = fdiv(row, a.fd_group);
+    float ro[D / 64], rm, rl;
+    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row - i * a.group, i, k_begin,
+                              min(k_end, visible(a, x, i)), rm, rl, ro);
+    store_row<Tag, D>(a, it, kv_head, row, first + b, ROWS, rm, rl, ro);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Many rows: WAVES waves of 32 rows each over blocks of 64 keys that they share.
+// Many rows: four waves of 32 rows each over blocks of 64 keys that they share.
 //
 // Scores are taken transposed, S^T = K Q^T with 32x32x16 products: a lane then
 // holds 32 keys' scores of one row (column lane % 32, keys 8 a + 4 (lane / 32)
@@ -483,10 +629,10 @@ constexpr float kLazyMax = 8.f;
 // K and V blocks go straight from global memory to LDS, one block ahead of
 // their use; one barrier a block.
 // ---------------------------------------------------------------------------
-template <class Tag, int D, int WAVES, bool PAGED>
-__global__ __launch_bounds__(WAVES * kWave, D <= 128 ? 2 : 1) void attn_tiles_kernel(
-    const AttnArgs a) {
-  constexpr int ROWS = WAVES * 32;
+template <class Tag, int D, Keys KEYS>
+__global__ __launch_bounds__(kBlock, D <= 128 ? 2 : 1) void attn_tiles_kernel(const AttnArgs a) {
+  constexpr bool PAGED = KEYS != Keys::kPacked;
+  constexpr int WAVES = kBlock / kWave, ROWS = kTileRows;
   constexpr int BLOCK = kKeyBlock * D * 2;  // bytes of a K or V block
   constexpr int PER = kWave / (D / 8);      // rows a load
   constexpr int COUNT = kKeyBlock / PER / WAVES;
@@ -541,148 +687,204 @@ __global__ __launch_bounds__(WAVES * kWave, D <= 128 ? 2 : 1) void attn_tiles_ke
 
   const char* kp = static_cast<const char*>(a.k) + kv_head * a.k_hs * Tag::kBytes;
   const char* vp = static_cast<const char*>(a.v) + kv_head * a.v_hs * Tag::kBytes;
-  const int first_row = wave * (kKeyBlock / WAVES);
-  auto load_block = [&](const KeyRows& kr, int buf) {
-    load_rows<D, COUNT, false>(kp, kr.k16, lds + buf * BLOCK, first_row, lane);
-    load_rows<D, COUNT, true>(vp, kr.v16, lds + (2 + buf) * BLOCK, first_row, lane);
+  const int n = (k_end - k_begin + kKeyBlock - 1) / kKeyBlock;  // blocks of the range
+  const int first_row = wave * (kKeyBlock / WAVES);             // of a block: this wave's loads
+  auto base_of = [&](int t) JO_INLINE { return k_begin + t * kKeyBlock; };
+  auto page_of_block = [&](int t) JO_INLINE {
+    return key_page<PAGED>(a, it.r, min(base_of(t), k_end - 1), k_end);
   };
 
-  const uint32_t k_addr = lds + (lane % 32) * (D * 2) + ((half ^ swz_k<D>(lane % 32)) << 4);
-  // Lane's place in V's transposing reads: key 4 half + i / 4 of a 16-key step,
-  // columns 16 (lane / 16 % 2) + 4 (i % 4) of a 32-column block (i = lane % 16).
-  const int vi = lane % 16;
-  const int v_row = half * 4 + vi / 4;
-  const int v_chunk = (lane / 16 % 2) * 2 + (vi % 4) / 2;
-  const uint32_t v_addr = lds + 2 * BLOCK + v_row * (D * 2) + (vi % 2) * 8;
-
-  if (k_begin < k_end) {
-    KeyRows cur = key_rows<PAGED>(a, x, key_page<PAGED>(a, it.r, k_begin, k_end), k_begin, k_end);
-    load_block(cur, 0);
-    int32_t next_page = k_begin + kKeyBlock < k_end
-                            ? key_page<PAGED>(a, it.r, k_begin + kKeyBlock, k_end)
-                            : 0;
-    int buf = 0;
-    for (int base = k_begin; base < k_end; base += kKeyBlock, buf ^= 1) {
-      // This block is in LDS (own loads: the wait; the other waves': the
-      // barrier), and every wave is done with the other buffer.
-      JO_KEEP_ORDER();
-      JO_WAIT_VM(0);
-      JO_WAIT_LDS0();
-      __builtin_amdgcn_s_barrier();
-      JO_KEEP_ORDER();
-      const uint64_t there = cur.there;
-      if (base + kKeyBlock < k_end) {
-        cur = key_rows<PAGED>(a, x, next_page, base + kKeyBlock, k_end);
-        load_block(cur, buf ^ 1);
-        if (base + 2 * kKeyBlock < k_end)
-          next_page = key_page<PAGED>(a, it.r, base + 2 * kKeyBlock, k_end);
+  // Where the wave's rows of a block are: one address (kPages16, kPacked), or an
+  // offset a key (kPages). Rows behind the range's last key read that key.
+  struct Rows {
+    KeyRows each;          // kPages; `there` in every mode
+    int64_t k_off, v_off;  // else: bytes to the row of key `from`
+    int from, last;        // of the block: keys from .. last are read by this wave
+  };
+  auto rows_of = [&](int t, int32_t page) JO_INLINE {
+    const int base = base_of(t);
+    Rows b;
+    if constexpr (KEYS == Keys::kPages) {
+      b.each = key_rows<true>(a, x, page, base, k_end);
+    } else {
+      b.last = min(kKeyBlock, k_end - base) - 1;
+      b.from = min(first_row, b.last & ~15);
+      uint32_t row = x.k0 + base + b.from;
+      int64_t p = 0;
+      b.each.there = ~uint64_t{0};
+      if constexpr (KEYS == Keys::kPages16) {
+        // (Lanes behind the range hold its last key's page.)
+        b.each.there = __ballot(page >= 0 && page < a.num_pages);
+        const int32_t mine = __builtin_amdgcn_readlane(page, b.from);
+        p = mine >= 0 && mine < a.num_pages ? mine : 0;
+        row -= fdiv(row, a.fd_page) * a.fd_page.d;
       }
-      if (base >= wave_end) continue;  // the wave's rows see none of these keys
-
-      f32x16 s[2] = {};
-      const uint32_t ka = k_addr + buf * BLOCK;
+      b.k_off = (p * a.k_ps16 + static_cast<int64_t>(row) * a.k_ts16) << 4;
+      b.v_off = (p * a.v_ps16 + static_cast<int64_t>(row) * a.v_ts16) << 4;
+      if (b.last < kKeyBlock - 1) b.each.there &= (uint64_t{2} << b.last) - 1;
+    }
+    return b;
+  };
+  // This wave's rows of K (V32 false) or V to LDS at `to`.
+  auto load_rows_of = [&](const Rows& b, auto v32, uint32_t to) JO_INLINE {
+    constexpr bool V32 = decltype(v32)::value;
+    if constexpr (KEYS == Keys::kPages) {
+      load_rows<D, COUNT, V32>(V32 ? vp : kp, V32 ? b.each.v16 : b.each.k16, to, first_row, lane);
+    } else {
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = mfma32<Tag>(lds_read16((ka ^ (k << 5)) + b * 32 * D * 2), q[k], s[b]);
-      }
-      if (base + kKeyBlock > first_end || ~there != 0) {  // uniform
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = b * 32 + (e / 4) * 8 + half * 4 + e % 4;
-            if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
-          }
-      }
-      float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
-      if (__any(top * a.scale_log2 > m + kLazyMax)) {
-        const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2);
-        const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-        m = m_new;
-        l *= fade;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= fade;
-      }
-      const float m_use = m == -INFINITY ? 0.f : m;
-      u32x4 p[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = exp2_fast(fmaf(s[k / 2][(k % 2) * 8 + e], a.scale_log2, -m_use));
-          l += w[e];
-        }
-        p[k] = u32x4{pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
-                     pack2<Tag>(w[6], w[7])};
-      }
-      const uint32_t va = v_addr + buf * BLOCK;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const uint32_t row = va + k * 16 * D * 2;
-          const int sw0 = swz_v32<D>(v_row), sw1 = swz_v32<D>(v_row + 8);
-          o[d] = mfma32<Tag>(lds_read_tr(row + (((d * 4 + v_chunk) ^ sw0) << 4),
-                                         row + 8 * D * 2 + (((d * 4 + v_chunk) ^ sw1) << 4)),
-                             p[k], o[d]);
-        }
+      for (int i = 0; i < COUNT; ++i) {
+        const int row = first_row + i * PER + lane / (D / 8);
+        const int chunk = (lane % (D / 8)) ^ (V32 ? swz_v32<D>(row) : swz_k<D>(row));
+        const uint32_t off = (min(row, b.last) - b.from) * (V32 ? a.v_ts16 : a.k_ts16) + chunk;
+        load_to_lds((V32 ? vp + b.v_off : kp + b.k_off), off << 4,
+                    to + (first_row + i * PER) * D * 2);
       }
     }
-  }
-  l += __shfl_xor(l, 32);
-
-  bool fine = true;
+  };
+  auto load_k = [&](const Rows& b, int buf) JO_INLINE {
+    load_rows_of(b, std::false_type{}, lds + buf * BLOCK);
+  };
+  auto load_v = [&](const Rows& b, int buf) JO_INLINE {
+    load_rows_of(b, std::true_type{}, lds + (2 + buf) * BLOCK);
+  };
+  // Lane addresses of the operand reads, one a 16-element step of head_dim (K)
+  // and one a 32-column block and half step (V); buffers, key steps and blocks
+  // are constants from there.
+  uint32_t k_addr[KK], v_addr[DB][2];
+#pragma unroll
+  for (int k = 0; k < KK; ++k)
+    k_addr[k] = lds + (lane % 32) * (D * 2) + (((2 * k + half) ^ swz_k<D>(lane % 32)) << 4);
+  // V's transposing reads: key 4 half + i / 4 of an 8-key half step, columns
+  // 16 (lane / 16 % 2) + 4 (i % 4) of a 32-column block (i = lane % 16).
+  const int v_row = half * 4 + lane % 16 / 4;
+  const int v_chunk = (lane / 16 % 2) * 2 + (lane % 4) / 2;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) fine = fine && all_finite(o[d][e]);
-  fine = fine && all_finite(l);
-  const uint64_t bad = __ballot(!fine && my_row < rows);
-  if (my_row < rows) {
-    if (it.splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      char* out = static_cast<char*>(a.out) +
-                  ((x.q0 + my_i) * a.o_ts + my_head * a.o_hs + half * 4) * Tag::kBytes;
+    for (int h = 0; h < 2; ++h)
+      v_addr[d][h] = lds + 2 * BLOCK + (v_row + 8 * h) * (D * 2) + (lane % 2) * 8 +
+                     (((d * 4 + v_chunk) ^ swz_v32<D>(v_row + 8 * h)) << 4);
+
+  f32x16 s[2];
+  u32x4 p[4];
+  auto other_buffer = [&](int buf) JO_INLINE {
+    const int step = buf ? -BLOCK : BLOCK;
+#pragma unroll
+    for (int k = 0; k < KK; ++k) k_addr[k] += step;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) v_addr[d][h] += step;
+  };
+  auto v_read = [&](int k, int d) JO_INLINE {
+    return lds_read_tr(v_addr[d][0] + k * 16 * D * 2, v_addr[d][1] + k * 16 * D * 2);
+  };
+  // Products in groups of four whose operands are read a group ahead: groups 0 ..
+  // DB - 1 are V^T P^T (four of the 16-key steps x 32-column blocks each), the
+  // KK / 2 groups behind them K Q^T (two steps of head_dim, two key halves).
+  auto read_group = [&](u32x4 (&f)[4], int g) JO_INLINE {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      f[e] = g < DB ? v_read((g * 4 + e) / DB, (g * 4 + e) % DB)
+                    : lds_read16(k_addr[(g - DB) * 2 + e / 2] + e % 2 * 32 * D * 2);
+  };
+  auto multiply_group = [&](const u32x4 (&f)[4], int g) JO_INLINE {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (g < DB)
+        o[(g * 4 + e) % DB] = mfma32<Tag>(f[e], p[(g * 4 + e) / DB], o[(g * 4 + e) % DB]);
+      else
+        s[e % 2] = mfma32<Tag>(f[e], q[(g - DB) * 2 + e / 2], s[e % 2]);
+    }
+  };
+  // From scores to weights in two parts: what this row has seen so far is scaled
+  // to a larger maximum, and the k-th 16 weights.
+  float m_use = 0.f;
+  auto new_max = [&](int t, uint64_t there) JO_INLINE {
+    const int base = base_of(t);
+    if (base + kKeyBlock > first_end || ~there != 0) {  // uniform
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = b * 32 + (e / 4) * 8 + half * 4 + e % 4;
+          if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = nan_max(top, s[e / 16][e % 16]);
+    if (__any(top * a.scale_log2 > m + kLazyMax)) {
+      const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2);
+      const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+      m = m_new;
+      l *= fade;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          st8(out + (d * 32 + e * 8) * Tag::kBytes,
-              u32x2{pack2<Tag>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
-                    pack2<Tag>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)});
-    } else {
-      float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
-      const int row = wave * 32 + lane % 32;
+        for (int e = 0; e < 16; ++e) o[d][e] *= fade;
+    }
+    m_use = m == -INFINITY ? 0.f : m;
+  };
+  auto weights = [&](int k) JO_INLINE {
+    float w[8];
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+    for (int e = 0; e < 8; ++e) {
+      w[e] = exp2_fast(fmaf(s[k / 2][(k % 2) * 8 + e], a.scale_log2, -m_use));
+      l += w[e];
+    }
+    p[k] = u32x4{pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
+                 pack2<Tag>(w[6], w[7])};
+  };
+  Rows next;
+  int32_t page = 0;
+  if (n > 0) {
+    next = rows_of(0, page_of_block(0));
+    load_k(next, 0);
+    load_v(next, 0);
+    page = page_of_block(1);
+  }
+  int buf = 0;
+  for (int t = 0; t < n; ++t, buf ^= 1) {
+    // This block is in LDS (this wave's loads: the wait; the others': the
+    // barrier), and every wave is done with the other buffer.
+    JO_KEEP_ORDER();
+    JO_WAIT_VM(0);
+    JO_WAIT_LDS0();
+    __builtin_amdgcn_s_barrier();
+    JO_KEEP_ORDER();
+    const uint64_t there = next.each.there;
+    if (t + 1 < n) {
+      next = rows_of(t + 1, page);
+      load_k(next, buf ^ 1);
+      load_v(next, buf ^ 1);
+      page = page_of_block(t + 2);
+    }
+    if (base_of(t) < wave_end) {  // else the wave's rows see none of these keys (uniform)
+      u32x4 f[2][4];
+      read_group(f[0], DB);
+      s[0] = s[1] = f32x16{};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<f32x4*>(part + row * D + d * 32 + e * 8 + half * 4) =
-              f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
-      if (half == 0) {
-        part[ROWS * D + row] = m;
-        part[ROWS * (D + 1) + row] = l;
+      for (int g = 0; g < KK / 2; ++g) {
+        read_group(f[(g + 1) % 2], g + 1 < KK / 2 ? DB + g + 1 : 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply_group(f[g % 2], DB + g);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      new_max(t, there);
+#pragma unroll
+      for (int g = 0; g < DB; ++g) {
+        if (g + 1 < DB) read_group(f[(KK / 2 + g + 1) % 2], g + 1);
+        // (Group g's products take the weights of its 16-key steps.)
+#pragma unroll
+        for (int k = (g * 4 + DB - 1) / DB; k < ((g + 1) * 4 + DB - 1) / DB; ++k) weights(k);
+        multiply_group(f[(KK / 2 + g) % 2], g);
       }
     }
+    other_buffer(buf);
   }
-  uint32_t again = static_cast<uint32_t>(bad) | static_cast<uint32_t>(bad >> 32);
-  while (again != 0) {
-    const int b = __builtin_ctz(again);
-    again &= again - 1;
-    const int row = row0 + wave * 32 + b;
-    const int i = fdiv(row, a.fd_group);
-    float ro[D / 64], rm, rl;
-    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row - i * a.group, i, k_begin,
-                              min(k_end, visible(a, x, i)), rm, rl, ro);
-    store_row<Tag, D>(a, it, kv_head, row, wave * 32 + b, ROWS, rm, rl, ro);
-  }
+  l += __shfl_xor(l, 32);
+  store_tile<Tag, D, ROWS, PAGED>(args_again(), it, kv_head, wave * 32, k_begin, k_end, o, m, l);
 }
 
 // ---------------------------------------------------------------------------
@@ -763,7 +965,7 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
 
   constexpr int STEP = W * S::kKeys;  // a wave's blocks are this far apart
   const int my_begin = k_begin + wave * S::kKeys;
-  auto attend = [&](int base, int buf, uint32_t there) {
+  auto attend = [&](int base, int buf, uint32_t there) JO_INLINE {
           f32x4 s[2] = {};
           const uint32_t ka = k_addr + buf * BLOCK;
     #pragma unroll
@@ -877,11 +1079,11 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
       for (int c = 0; c < 4; ++c) r[n][c] = fmaf(e, v[c], r[n][c]);
     }
   }
-  bool fine = all_finite(sum);
+  bool fine = finite_bits(sum);
 #pragma unroll
   for (int n = 0; n < NE; ++n)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) fine = fine && all_finite(r[n][c]);
+    for (int c = 0; c < 4; ++c) fine = fine && finite_bits(r[n][c]);
   const bool mine_row = row0 + row < rows;
   uint64_t bad = __ballot(!fine && mine_row);
   if (mine_row) {
@@ -917,41 +1119,76 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
   }
 }
 
-// Joins the partial results of split tiles: a workgroup a tile and key head.
-// out = sum_s e_s o_s / sum_s e_s l_s, e_s = 2^(m_s - max m).
-template <class Tag, int D, int ROWS, bool PAGED>
+// Joins the partial results of split tiles:
+//   out = sum_s e_s o_s / sum_s e_s l_s, e_s = 2^(m_s - max m).
+// A workgroup takes kBlock / (D / 4) / GROUPS rows of a tile and key head, four
+// elements a thread, the splits dealt out to GROUPS threads of each element
+// whose sums meet in LDS: with few rows there are many splits, and one thread
+// would wait for them one after the other.
+template <class Tag, int D, int ROWS, bool PAGED, int GROUPS>
 __global__ __launch_bounds__(kBlock) void attn_join_kernel(const AttnArgs a) {
-  const uint32_t tile_id = blockIdx.x / a.kv_heads;
-  const int kv_head = blockIdx.x - tile_id * a.kv_heads;
+  constexpr int C = D / 4;                    // threads a row and group
+  constexpr int PER = kBlock / C / GROUPS;    // rows a workgroup
+  constexpr int PARTS = ROWS / PER;
+  const uint32_t unit = blockIdx.x / PARTS;
+  const int row0 = (blockIdx.x % PARTS) * PER;
+  const uint32_t tile_id = unit / a.kv_heads;
+  const int kv_head = unit - tile_id * a.kv_heads;
   const Item it = find_item<ROWS, PAGED, true>(a, tile_id);
   // (A last item that was not launched: lengths that overlap, nothing to join.)
   if (it.r < 0 || it.splits == 1 || static_cast<uint32_t>(it.index + it.splits) > a.items) return;
   const int rows = min(ROWS, it.x.nq * a.group - it.tile * ROWS);
+  if (row0 >= rows) return;
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * ROWS * (D + 2);
   const float* first = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
-  constexpr int C = D / 4;  // threads a row
-  for (int at = threadIdx.x; at < rows * C; at += kBlock) {
-    const int row = at / C, c = at % C;
-    float top = -INFINITY;
-    for (int s = 0; s < it.splits; ++s) top = fmaxf(top, first[s * stride + ROWS * D + row]);
-    float sum = 0.f;
-    f32x4 r = {};
-    for (int s = 0; s < it.splits; ++s) {
-      const float* p = first + s * stride;
-      const float ms = p[ROWS * D + row], ls = p[ROWS * (D + 1) + row];
-      if (ms == -INFINITY && ls == 0.f) continue;  // sees none of this range
-      const float e = exp2_fast(ms - top);
-      sum = fmaf(e, ls, sum);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(p + row * D + c * 4);
+  const int c = threadIdx.x % C, group = threadIdx.x / C % GROUPS;
+  const int row = min(row0 + static_cast<int>(threadIdx.x) / (C * GROUPS), rows - 1);
+  float top = -INFINITY, sum = 0.f;
+  f32x4 r = {};
+#pragma unroll 4
+  for (int s = group; s < it.splits; s += GROUPS) {
+    const float* p = first + s * stride;
+    const float ms = p[ROWS * D + row], ls = p[ROWS * (D + 1) + row];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p + row * D + c * 4);
+    const float m_new = fmaxf(top, ms);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float fade = exp2_fast(top - m_use), e = exp2_fast(ms - m_use);
+    top = m_new;
+    sum = fmaf(e, ls, sum * fade);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k] * fade);
+  }
+  if constexpr (GROUPS > 1) {
+    __shared__ f32x4 s_r[kBlock];
+    __shared__ float s_m[kBlock], s_l[kBlock];
+    s_r[threadIdx.x] = r;
+    s_m[threadIdx.x] = top;
+    s_l[threadIdx.x] = sum;
+    __syncthreads();
+    if (group != 0) return;
+    const int at = threadIdx.x;
+    float all = top;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) all = fmaxf(all, s_m[at + g * C]);
+    const float use = all == -INFINITY ? 0.f : all;
+    sum = 0.f;
+    r = f32x4{};
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const float e = exp2_fast(s_m[at + g * C] - use);
+      const f32x4 v = s_r[at + g * C];
+      sum = fmaf(e, s_l[at + g * C], sum);
 #pragma unroll
       for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k]);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int i = fdiv(it.tile * ROWS + row, a.fd_group);
-    const int head = kv_head * a.group + it.tile * ROWS + row - i * a.group;
-    st8(byte_off(a.out, ((it.x.q0 + i) * a.o_ts + head * a.o_hs + c * 4) * Tag::kBytes),
-        u32x2{pack2<Tag>(r[0] * inv, r[1] * inv), pack2<Tag>(r[2] * inv, r[3] * inv)});
   }
+  const int at_row = it.tile * ROWS + row0 + static_cast<int>(threadIdx.x) / (C * GROUPS);
+  if (at_row >= it.x.nq * a.group) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int i = fdiv(at_row, a.fd_group);
+  const int head = kv_head * a.group + at_row - i * a.group;
+  st8(byte_off(a.out, ((it.x.q0 + i) * a.o_ts + head * a.o_hs + c * 4) * Tag::kBytes),
+      u32x2{pack2<Tag>(r[0] * inv, r[1] * inv), pack2<Tag>(r[2] * inv, r[3] * inv)});
 }
 
 // ---------------------------------------------------------------------------
@@ -965,7 +1202,8 @@ struct AttnPlan {
   int64_t ws_bytes;
 };
 
-constexpr int kTileWaves = 4;
+constexpr int64_t kComputeUnits = 256;
+constexpr int kFewJoin = 4, kTileJoin = 1;  // threads that share an element's splits
 
 AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                         int64_t head_dim, int64_t kv_capacity) {
@@ -973,14 +1211,17 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   const int64_t group = q_heads / kv_heads;
   const int64_t all_rows = q_tokens * group;
   p.few = all_rows <= 16 * requests;
-  const int64_t rows = p.few ? 16 : 32 * kTileWaves;
+  const int64_t rows = p.few ? 16 : kTileRows;
   p.tiles = all_rows / rows + (requests < q_tokens || requests > kPlanRequests ? requests : q_tokens);
   if (requests == 0) p.tiles = 0;
   const int64_t blocks = (kv_capacity + kKeyBlock - 1) / kKeyBlock;
-  const int64_t groups = p.tiles * kv_heads;
+  // Workgroups that run at once: LDS and registers let two of the smaller ones
+  // share a compute unit.
+  const int64_t slots = kComputeUnits * (p.few ? (head_dim == 64 ? 2 : 1) : (head_dim <= 128 ? 2 : 1));
+  const int64_t round = (slots + kv_heads - 1) / kv_heads;  // items of one round
   p.split_target = 0;
-  if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && groups < 1024)
-    p.split_target = (1024 + kv_heads - 1) / kv_heads;
+  if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && p.tiles < 8 * round)
+    p.split_target = p.tiles <= round / 2 ? round - p.tiles : p.few ? 2 * round : round;
   const int64_t most = p.tiles * (blocks / kMinChunk + 1);
   p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;
   p.ws_bytes = p.split_target == 0 ? 0 : p.items * kv_heads * rows * (head_dim + 2) * 4;
@@ -997,6 +1238,7 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
     p.items = p.tiles;
   }
   a.split_target = static_cast<uint32_t>(p.split_target);
+  a.fd_target = make_fastdiv(a.split_target);
   a.items = static_cast<uint32_t>(p.items);
   a.ws = static_cast<float*>(ws);
   // Workgroups that clear the rows of no request, 64 KB each if they are all.
@@ -1009,16 +1251,26 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
   if (p.few)
     hipLaunchKernelGGL((attn_few_kernel<Tag, D, PAGED>), grid, dim3(FewShape<D>::kWaves * kWave), 0,
                        stream, a);
+  else if constexpr (!PAGED)
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPacked>), grid, dim3(kBlock), 0, stream, a);
+  else if (a.fd_page.d % 16 == 0)
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages16>), grid, dim3(kBlock), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, kTileWaves, PAGED>), grid,
-                       dim3(kTileWaves * kWave), 0, stream, a);
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages>), grid, dim3(kBlock), 0, stream, a);
   int st = launch_status(op);
   if (st != JO_OK || p.split_target == 0) return st;
-  const dim3 join(static_cast<unsigned>(p.tiles * a.kv_heads));
+  // Tiles that are split: no more than split_target, since each has more key
+  // blocks than a chunk.
+  const int64_t split_tiles = p.tiles < p.split_target ? p.tiles : p.split_target;
+  const int64_t joins = split_tiles * a.kv_heads * (p.few ? 16 : kTileRows) * (D / 4) *
+                        (p.few ? kFewJoin : kTileJoin) / kBlock;
+  JO_REQUIRE(joins <= INT32_MAX / 512, "%s: shape too large", op);
+  const dim3 join(static_cast<unsigned>(joins));
   if (p.few)
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED>), join, dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED, kFewJoin>), join, dim3(kBlock), 0, stream,
+                       a);
   else
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 32 * kTileWaves, PAGED>), join, dim3(kBlock), 0,
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, kTileRows, PAGED, kTileJoin>), join, dim3(kBlock), 0,
                        stream, a);
   return launch_status(op);
 }
@@ -1089,6 +1341,8 @@ int key_offsets(const char* op, AttnArgs& a, int64_t pages, int64_t rows) {
     const int64_t ps = i ? a.v_ps : a.k_ps, ts = i ? a.v_ts : a.k_ts;
     JO_REQUIRE((reach(pages, ps) + reach(rows, ts)) / 8 <= INT32_MAX * int64_t{2},
                "%s: K and V rows must lie within 64 GiB", op);
+    // (64 rows' offsets in 32 bits of bytes.)
+    JO_REQUIRE(ts < (int64_t{1} << 24), "%s: token stride of K or V too large", op);
     (i ? a.v_ps16 : a.k_ps16) = static_cast<uint32_t>(pages > 1 ? ps / 8 : 0);
     (i ? a.v_ts16 : a.k_ts16) = static_cast<uint32_t>(rows > 1 ? ts / 8 : 0);
   }
