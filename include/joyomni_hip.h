@@ -527,8 +527,9 @@ int jo_kv_commit_rope(const void* src_k, const void* src_v, void* dst_k, void* d
  *   *free_left = *num_free - pages taken (negative: so many are missing)
  * *num_free counts as at most free_capacity. The stack itself is only read: the
  * next step's *num_free is *free_left when pages were not missing. Sizes of
- * outputs: cu_q requests + 1, kv_lens requests, slots max_tokens. requests <=
- * 4096. */
+ * outputs: cu_q requests + 1, kv_lens requests, slots max_tokens. No output
+ * (block_table among them) overlaps an input or another output: kv_lens is not
+ * ctx_lens itself. requests <= 4096. */
 int jo_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens, int64_t requests,
                     int32_t* block_table, int64_t table_stride, int64_t table_width,
                     const int32_t* free_pages, int64_t free_capacity, const int32_t* num_free,
@@ -570,8 +571,13 @@ int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, void* pages_k,
  *     are not seen.
  * q, out: [q_tokens, q_heads, head_dim]. All strides in elements, multiples of
  * 8, tensors 16-byte aligned, head_dim contiguous: 64, 128 or 256. dtype bf16 or
- * fp16, q_heads a multiple of kv_heads, scale > 0. out overlaps no input.
- * cu_q, cu_k: int32 [requests + 1], non-decreasing from 0 on.
+ * fp16, q_heads a multiple of kv_heads (65536 at most), 0 < scale <= 1e30. out
+ * overlaps no input, its rows not each other: one of its strides steps over all
+ * that the other one reaches. Strides of K and V are not negative, of tokens
+ * below 2^24 elements, and every row of K and V begins within 64 GiB of its
+ * tensor's start; q_tokens * q_heads < 2^30.
+ * cu_q, cu_k: int32 [requests + 1], non-decreasing from 0 on (values that are
+ * not give results without meaning, inside the tensors all the same).
  * The workspace (jo_attention_workspace_bytes, 16-byte aligned; NULL with 0
  * bytes: keys are not split) holds partial results of split key ranges; it is
  * in use until the work queued on `stream` finishes. */
@@ -596,7 +602,7 @@ int jo_attention_paged(const void* q, const void* pages_k, const void* pages_v, 
 
 /* Workspace bytes that the two calls above use for these sizes (0: none);
  * kv_capacity is kv_tokens, or table_width * page_size. A host-side
- * computation. */
+ * computation; a few hundred MB at most. */
 int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests, int64_t q_heads,
                                      int64_t kv_heads, int64_t head_dim, int64_t kv_capacity);
 

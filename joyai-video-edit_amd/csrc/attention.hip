@@ -1121,74 +1121,77 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
 
 // Joins the partial results of split tiles:
 //   out = sum_s e_s o_s / sum_s e_s l_s, e_s = 2^(m_s - max m).
-// A workgroup takes kBlock / (D / 4) / GROUPS rows of a tile and key head, four
-// elements a thread, the splits dealt out to GROUPS threads of each element
-// whose sums meet in LDS: with few rows there are many splits, and one thread
-// would wait for them one after the other.
-template <class Tag, int D, int ROWS, bool PAGED, int GROUPS>
+// A workgroup takes EACH times kBlock / (D / 4) / GROUPS rows of a tile and key
+// head, four elements a thread, the splits dealt out to GROUPS threads of each
+// element whose sums meet in LDS: with few rows there are many splits, and one
+// thread would wait for them one after the other.
+template <class Tag, int D, int ROWS, bool PAGED, int GROUPS, int EACH>
 __global__ __launch_bounds__(kBlock) void attn_join_kernel(const AttnArgs a) {
   constexpr int C = D / 4;                    // threads a row and group
   constexpr int PER = kBlock / C / GROUPS;    // rows a workgroup
-  constexpr int PARTS = ROWS / PER;
+  static_assert(GROUPS == 1 || EACH == 1, "the rows' sums in LDS are for one step");
+  constexpr int PARTS = ROWS / PER / EACH;
   const uint32_t unit = blockIdx.x / PARTS;
-  const int row0 = (blockIdx.x % PARTS) * PER;
+  const int row_begin = (blockIdx.x % PARTS) * PER * EACH;
   const uint32_t tile_id = unit / a.kv_heads;
   const int kv_head = unit - tile_id * a.kv_heads;
   const Item it = find_item<ROWS, PAGED, true>(a, tile_id);
   // (A last item that was not launched: lengths that overlap, nothing to join.)
   if (it.r < 0 || it.splits == 1 || static_cast<uint32_t>(it.index + it.splits) > a.items) return;
   const int rows = min(ROWS, it.x.nq * a.group - it.tile * ROWS);
-  if (row0 >= rows) return;
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * ROWS * (D + 2);
   const float* first = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
   const int c = threadIdx.x % C, group = threadIdx.x / C % GROUPS;
-  const int row = min(row0 + static_cast<int>(threadIdx.x) / (C * GROUPS), rows - 1);
-  float top = -INFINITY, sum = 0.f;
-  f32x4 r = {};
+#pragma unroll 1
+  for (int row0 = row_begin; row0 < min(rows, row_begin + PER * EACH); row0 += PER) {
+    const int row = min(row0 + static_cast<int>(threadIdx.x) / (C * GROUPS), rows - 1);
+    float top = -INFINITY, sum = 0.f;
+    f32x4 r = {};
 #pragma unroll 4
-  for (int s = group; s < it.splits; s += GROUPS) {
-    const float* p = first + s * stride;
-    const float ms = p[ROWS * D + row], ls = p[ROWS * (D + 1) + row];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(p + row * D + c * 4);
-    const float m_new = fmaxf(top, ms);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float fade = exp2_fast(top - m_use), e = exp2_fast(ms - m_use);
-    top = m_new;
-    sum = fmaf(e, ls, sum * fade);
+    for (int s = group; s < it.splits; s += GROUPS) {
+      const float* p = first + s * stride;
+      const float ms = p[ROWS * D + row], ls = p[ROWS * (D + 1) + row];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(p + row * D + c * 4);
+      const float m_new = fmaxf(top, ms);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float fade = exp2_fast(top - m_use), e = exp2_fast(ms - m_use);
+      top = m_new;
+      sum = fmaf(e, ls, sum * fade);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k] * fade);
-  }
-  if constexpr (GROUPS > 1) {
-    __shared__ f32x4 s_r[kBlock];
-    __shared__ float s_m[kBlock], s_l[kBlock];
-    s_r[threadIdx.x] = r;
-    s_m[threadIdx.x] = top;
-    s_l[threadIdx.x] = sum;
-    __syncthreads();
-    if (group != 0) return;
-    const int at = threadIdx.x;
-    float all = top;
-#pragma unroll
-    for (int g = 1; g < GROUPS; ++g) all = fmaxf(all, s_m[at + g * C]);
-    const float use = all == -INFINITY ? 0.f : all;
-    sum = 0.f;
-    r = f32x4{};
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const float e = exp2_fast(s_m[at + g * C] - use);
-      const f32x4 v = s_r[at + g * C];
-      sum = fmaf(e, s_l[at + g * C], sum);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k]);
+      for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k] * fade);
     }
+    if constexpr (GROUPS > 1) {
+      __shared__ f32x4 s_r[kBlock];
+      __shared__ float s_m[kBlock], s_l[kBlock];
+      s_r[threadIdx.x] = r;
+      s_m[threadIdx.x] = top;
+      s_l[threadIdx.x] = sum;
+      __syncthreads();
+      if (group != 0) return;
+      const int at = threadIdx.x;
+      float all = top;
+#pragma unroll
+      for (int g = 1; g < GROUPS; ++g) all = fmaxf(all, s_m[at + g * C]);
+      const float use = all == -INFINITY ? 0.f : all;
+      sum = 0.f;
+      r = f32x4{};
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        const float e = exp2_fast(s_m[at + g * C] - use);
+        const f32x4 v = s_r[at + g * C];
+        sum = fmaf(e, s_l[at + g * C], sum);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = fmaf(e, v[k], r[k]);
+      }
+    }
+    const int at_row = it.tile * ROWS + row0 + static_cast<int>(threadIdx.x) / (C * GROUPS);
+    if (at_row >= it.x.nq * a.group) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int i = fdiv(at_row, a.fd_group);
+    const int head = kv_head * a.group + at_row - i * a.group;
+    st8(byte_off(a.out, ((it.x.q0 + i) * a.o_ts + head * a.o_hs + c * 4) * Tag::kBytes),
+        u32x2{pack2<Tag>(r[0] * inv, r[1] * inv), pack2<Tag>(r[2] * inv, r[3] * inv)});
   }
-  const int at_row = it.tile * ROWS + row0 + static_cast<int>(threadIdx.x) / (C * GROUPS);
-  if (at_row >= it.x.nq * a.group) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int i = fdiv(at_row, a.fd_group);
-  const int head = kv_head * a.group + at_row - i * a.group;
-  st8(byte_off(a.out, ((it.x.q0 + i) * a.o_ts + head * a.o_hs + c * 4) * Tag::kBytes),
-      u32x2{pack2<Tag>(r[0] * inv, r[1] * inv), pack2<Tag>(r[2] * inv, r[3] * inv)});
 }
 
 // ---------------------------------------------------------------------------
@@ -1203,7 +1206,11 @@ struct AttnPlan {
 };
 
 constexpr int64_t kComputeUnits = 256;
-constexpr int kFewJoin = 4, kTileJoin = 1;  // threads that share an element's splits
+// Threads that share an element's splits, and steps of rows a workgroup takes.
+// (Tiles, 16384 rows a key head and less: two steps 89.3 us, one 91.9, four 90.3
+// for 20 requests of chunks and single tokens, the whole call; 62.5, 64.1, 62.1
+// for four prompts of 1000 tokens.)
+constexpr int kFewJoin = 4, kTileJoin = 1, kTileEach = 2;  // threads that share an element's splits
 
 AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                         int64_t head_dim, int64_t kv_capacity) {
@@ -1263,14 +1270,14 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
   // blocks than a chunk.
   const int64_t split_tiles = p.tiles < p.split_target ? p.tiles : p.split_target;
   const int64_t joins = split_tiles * a.kv_heads * (p.few ? 16 : kTileRows) * (D / 4) *
-                        (p.few ? kFewJoin : kTileJoin) / kBlock;
+                        (p.few ? kFewJoin : kTileJoin) / kBlock / (p.few ? 1 : kTileEach);
   JO_REQUIRE(joins <= INT32_MAX / 512, "%s: shape too large", op);
   const dim3 join(static_cast<unsigned>(joins));
   if (p.few)
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED, kFewJoin>), join, dim3(kBlock), 0, stream,
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED, kFewJoin, 1>), join, dim3(kBlock), 0, stream,
                        a);
   else
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, kTileRows, PAGED, kTileJoin>), join, dim3(kBlock), 0,
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, kTileRows, PAGED, kTileJoin, kTileEach>), join, dim3(kBlock), 0,
                        stream, a);
   return launch_status(op);
 }
@@ -1312,7 +1319,13 @@ int check_attention(const char* op, AttnArgs& a, const void* q, const void* k, c
                  (a.q_ts | a.q_hs | a.k_ps | a.k_ts | a.k_hs | a.v_ps | a.v_ts | a.v_hs | a.o_ts |
                   a.o_hs) % 8 == 0,
              "%s: strides must be multiples of 8 elements", op);
-  JO_REQUIRE((q_tokens <= 1 || a.o_ts >= head_dim) && (q_heads <= 1 || a.o_hs >= head_dim),
+  // One of out's strides steps over all that the other one reaches.
+  auto steps_over = [&](int64_t outer, int64_t n, int64_t inner) {
+    return n <= 1 || (outer >= head_dim && (outer - head_dim) / (n - 1) >= inner);
+  };
+  JO_REQUIRE((q_tokens <= 1 || a.o_ts >= head_dim) && (q_heads <= 1 || a.o_hs >= head_dim) &&
+                 (q_tokens <= 1 || q_heads <= 1 || steps_over(a.o_ts, q_heads, a.o_hs) ||
+                  steps_over(a.o_hs, q_tokens, a.o_ts)),
              "%s: rows of out must not overlap", op);
   a.q = q;
   a.k = k;

@@ -10,9 +10,9 @@
 //   table[r, have[r] + j] = free[num_free - 1 - base[r] - j]   (j < need[r] - have[r])
 //   slot[t] = table[r, p / P] * P + p % P,  p = ctx[r] + t - cu[r]
 //
-// Every workgroup scans all requests itself (two prefix sums, 1024 requests a
-// pass, the results in LDS) and then takes its share of the tokens and of the
-// new table entries: a token's new page is worked out from the free list, not
+// Every workgroup scans all requests itself (two prefix sums, a request a
+// thread and pass, the results in LDS) and then takes its share of the tokens and
+// of the new table entries: a token's new page is worked out from the free list, not
 // read back from the table, so workgroups wait for nobody and one launch does
 // it all. The work is a few KB; what it costs is the chain of latencies
 // (lengths, two scans, a search in LDS, a page id, the store).
@@ -23,9 +23,7 @@
 namespace jo {
 namespace {
 
-constexpr int kTabThreads = 1024;
-constexpr int kTabWaves = kTabThreads / kWave;
-constexpr int64_t kTabMaxRequests = 4096;  // cu and base in LDS: 8 bytes a request
+constexpr int64_t kTabMaxRequests = 4096;  // ctx, cu and base in LDS: 12 bytes a request
 
 struct TablesArgs {
   const int32_t* ctx;
@@ -49,28 +47,41 @@ __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
   return __builtin_elementwise_add_sat(a, b);
 }
 
-// Exclusive prefix sum over the workgroup's threads; `total` gets the sum.
+// Inclusive prefix sum over the wave, with DPP: shifts within rows of 16 lanes,
+// then the rows' totals handed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+  return add_sat(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL,
+                                                                      ROWS, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = scan_step<0x111, 0xf>(v);  // row_shr:1
+  v = scan_step<0x112, 0xf>(v);  // row_shr:2
+  v = scan_step<0x114, 0xf>(v);  // row_shr:4
+  v = scan_step<0x118, 0xf>(v);  // row_shr:8
+  v = scan_step<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  return scan_step<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+}
+
+// Prefix sum over the workgroup's threads (this thread's value left out);
+// `total` gets the sum.
+template <int WAVES>
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wave_sums, uint32_t& total) {
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  uint32_t s = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint32_t up = __shfl_up(s, d);
-    if (lane >= d) s = add_sat(s, up);
-  }
-  const uint32_t before_lane = __shfl_up(s, 1);
+  const uint32_t s = wave_scan(v);
+  const uint32_t up = __shfl_up(s, 1);
   if (lane == kWave - 1) wave_sums[wave] = s;
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kTabWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const uint32_t x = wave_sums[w];
     if (w < wave) before = add_sat(before, x);
     all = add_sat(all, x);
   }
   __syncthreads();
   total = all;
-  return add_sat(before, lane == 0 ? 0 : before_lane);
+  return add_sat(before, lane == 0 ? 0 : up);
 }
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, const TablesArgs& a) {
@@ -99,16 +110,19 @@ __device__ __forceinline__ uint32_t last_not_above(const uint32_t* key, uint32_t
   return lo;
 }
 
-__global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(const TablesArgs a) {
-  extern __shared__ uint32_t smem[];  // cu [requests + 1], base [requests + 1]
-  __shared__ uint32_t wave_sums[kTabWaves];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_tables_kernel(const TablesArgs a) {
+  extern __shared__ uint32_t smem[];  // cu [requests + 1], base [requests + 1], ctx [requests]
+  __shared__ uint32_t wave_sums[THREADS / kWave];
   uint32_t* cu = smem;
-  uint32_t* base = smem + a.requests + 1;
+  uint32_t* base = cu + a.requests + 1;
+  uint32_t* ctx_of = base + a.requests + 1;
   const uint32_t tid = threadIdx.x;
   const bool first = blockIdx.x == 0;
+  const int64_t available = min(max(a.num_free[0], 0), static_cast<int32_t>(a.free_capacity));
 
   uint32_t tokens = 0, pages = 0;  // of the requests before this pass
-  for (uint32_t r0 = 0; r0 < a.requests; r0 += kTabThreads) {
+  for (uint32_t r0 = 0; r0 < a.requests; r0 += THREADS) {
     const uint32_t r = r0 + tid;
     uint32_t ctx = 0, n = 0;
     if (r < a.requests) {
@@ -116,13 +130,15 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(const TablesA
       n = max(a.fresh[r], 0);
     }
     uint32_t sum;
-    const uint32_t at = min(add_sat(tokens, block_scan(n, wave_sums, sum)), a.max_tokens);
+    const uint32_t at =
+        min(add_sat(tokens, block_scan<THREADS / kWave>(n, wave_sums, sum)), a.max_tokens);
     const uint32_t end = min(add_sat(at, n), a.max_tokens);
     tokens = add_sat(tokens, sum);
     const uint32_t kv = ctx + (end - at);  // below 2^32: both are below 2^31
     const uint32_t have = pages_of(ctx, a), need = pages_of(kv, a);
-    const uint32_t mine = block_scan(need - have, wave_sums, sum);
+    const uint32_t mine = block_scan<THREADS / kWave>(need - have, wave_sums, sum);
     if (r < a.requests) {
+      ctx_of[r] = ctx;
       cu[r] = at;
       base[r] = add_sat(pages, mine);
       if (first) {
@@ -133,7 +149,6 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(const TablesA
     pages = add_sat(pages, sum);
   }
   tokens = min(tokens, a.max_tokens);
-  const int64_t available = min(max(a.num_free[0], 0), static_cast<int32_t>(a.free_capacity));
   if (tid == 0) {
     cu[a.requests] = tokens;
     base[a.requests] = pages;
@@ -145,13 +160,13 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(const TablesA
   }
   __syncthreads();
 
-  const uint64_t step = static_cast<uint64_t>(gridDim.x) * kTabThreads;
-  const uint64_t me = static_cast<uint64_t>(blockIdx.x) * kTabThreads + tid;
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * THREADS;
+  const uint64_t me = static_cast<uint64_t>(blockIdx.x) * THREADS + tid;
   for (uint64_t t = me; t < a.max_tokens; t += step) {
     int64_t slot = -1;
     if (t < tokens) {
       const uint32_t r = last_not_above(cu, a.requests, static_cast<uint32_t>(t));
-      const uint32_t ctx = max(a.ctx[r], 0);
+      const uint32_t ctx = ctx_of[r];
       const uint32_t pos = ctx + (static_cast<uint32_t>(t) - cu[r]);
       const uint32_t col = fdiv(pos, a.fd_page);
       if (col < a.width) {
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(const TablesA
   for (uint64_t i = me; i < pages; i += step) {
     const uint32_t r = last_not_above(base, a.requests, static_cast<uint32_t>(i));
     const uint32_t j = static_cast<uint32_t>(i) - base[r];
-    const uint32_t have = pages_of(max(a.ctx[r], 0), a);
+    const uint32_t have = pages_of(ctx_of[r], a);
     // (Bounded by the width also where a sum of pages has saturated.)
     if (j < a.width - have)
       a.table[static_cast<int64_t>(r) * a.table_stride + have + j] = take_page(a, available, i);
@@ -199,22 +214,46 @@ extern "C" int jo_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens,
   JO_REQUIRE(table_width <= INT32_MAX && free_capacity <= INT32_MAX && num_pages <= INT32_MAX &&
                  max_tokens <= INT32_MAX,
              "%s: shape too large", op);
-  JO_REQUIRE(requests <= 1 || table_stride >= table_width, "%s: bad table stride", op);
+  JO_REQUIRE(requests <= 1 || (table_stride >= table_width && table_stride <= int64_t{1} << 40),
+             "%s: bad table stride", op);
   JO_REQUIRE(cu_q && free_left && num_free, "%s: null pointer", op);
   JO_REQUIRE(free_left != num_free, "%s: free_left must not be num_free itself", op);
   JO_REQUIRE(requests == 0 || (ctx_lens && new_lens && kv_lens), "%s: null pointer", op);
   JO_REQUIRE(requests == 0 || table_width == 0 || block_table, "%s: null pointer", op);
   JO_REQUIRE((max_tokens == 0 || slots) && (free_capacity == 0 || free_pages), "%s: null pointer",
              op);
+  // Each workgroup reads all lengths and its part of the list, and what one has
+  // written another may not have read yet: no output lies in an input, not even
+  // kv_lens in ctx_lens.
+  const struct {
+    const void* p;
+    int64_t bytes;
+  } inputs[] = {{ctx_lens, 4 * requests}, {new_lens, 4 * requests},
+                {free_pages, 4 * free_capacity}, {num_free, 4}},
+    outputs[] = {{cu_q, 4 * (requests + 1)}, {kv_lens, 4 * requests}, {slots, 8 * max_tokens},
+                 {free_left, 4}, {block_table, requests == 0 || table_width == 0 ? 0
+                                  : 4 * ((requests - 1) * table_stride + table_width)}};
+  for (const auto& o : outputs)
+    for (const auto& i : inputs) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(o.p), y = reinterpret_cast<uintptr_t>(i.p);
+      JO_REQUIRE(o.bytes == 0 || i.bytes == 0 || x + o.bytes <= y || y + i.bytes <= x,
+                 "%s: an output overlaps an input", op);
+    }
   TablesArgs a{ctx_lens, new_lens, block_table, free_pages, num_free, cu_q, kv_lens, slots,
                free_left, table_stride, num_pages, static_cast<uint32_t>(requests),
                static_cast<uint32_t>(table_width), static_cast<uint32_t>(free_capacity),
                static_cast<uint32_t>(max_tokens), make_fastdiv(static_cast<uint32_t>(page_size))};
-  // A thread a token up to 64 workgroups, more tokens a thread beyond them.
-  const int64_t want = (max_tokens + kTabThreads - 1) / kTabThreads;
-  const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want > 64 ? 64 : want);
-  const size_t lds = 2 * (static_cast<size_t>(requests) + 1) * sizeof(uint32_t);
-  hipLaunchKernelGGL(paged_tables_kernel, dim3(grid), dim3(kTabThreads), lds,
-                     static_cast<hipStream_t>(stream), a);
+  // Few requests: four waves a workgroup, whose barriers cost less (32 requests in
+  // a replayed graph: 3.6 us a call, with 16 waves 4.8). Up to 64 workgroups of a
+  // thread a token; beyond them a thread takes more tokens.
+  const int64_t threads = requests <= 256 ? 256 : 1024;
+  const int64_t want = (max_tokens + threads - 1) / threads;
+  const dim3 grid(static_cast<unsigned>(want < 1 ? 1 : want > 64 ? 64 : want));
+  const size_t lds = (3 * static_cast<size_t>(requests) + 2) * sizeof(uint32_t);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (threads == 256)
+    hipLaunchKernelGGL((paged_tables_kernel<256>), grid, dim3(256), lds, st, a);
+  else
+    hipLaunchKernelGGL((paged_tables_kernel<1024>), grid, dim3(1024), lds, st, a);
   return launch_status(op);
 }

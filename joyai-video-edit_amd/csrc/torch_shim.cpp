@@ -12,6 +12,7 @@
 // carry the CUDA device type, so the impls are registered on the CUDA
 // dispatch key like the reference's. Every op runs
 // on the current stream of the tensor's device and never synchronizes.
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/all.h>
@@ -1078,10 +1079,13 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> paged_tab
   const int64_t ts = check_table(block_table, dev, R);
   TORCH_CHECK(max_tokens >= 0 && max_tokens <= INT32_MAX, "max_tokens must be in [0, 2^31)");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
-  auto cu = torch::empty({R + 1}, ctx_lens.options());
-  auto kv = torch::empty({R}, ctx_lens.options());
-  auto slots = torch::empty({max_tokens}, ctx_lens.options().dtype(torch::kInt64));
-  auto left = torch::empty({1}, ctx_lens.options());
+  // Allocated without the dispatcher's turn: four of those cost more host time
+  // than the kernel takes.
+  const auto i32 = ctx_lens.options();
+  const torch::Tensor cu = at::detail::empty_cuda({R + 1}, i32);
+  const torch::Tensor kv = at::detail::empty_cuda({R}, i32);
+  const torch::Tensor slots = at::detail::empty_cuda({max_tokens}, i32.dtype(torch::kInt64));
+  const torch::Tensor left = at::detail::empty_cuda({1}, i32);
   check_status(
       jo_paged_tables(ctx_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), R,
                       block_table.data_ptr<int32_t>(), ts, block_table.size(1),

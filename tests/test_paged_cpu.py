@@ -73,6 +73,18 @@ REFUSED = [
 ]
 
 
+REFUSED += [
+    # Rows of out that share elements without being too close one by one.
+    (varlen(ot=256, oh=128), "overlap"), (varlen(ot=128, oh=256), "overlap"),
+    (paged(ot=392, oh=128), "overlap"), (varlen(ot=128, oh=504), "overlap"),
+    # Rows of K and V that 32 bits do not reach.
+    (varlen(kt=2 ** 24), "stride"), (paged(vp=2 ** 36, N=8), "64 GiB"),
+    # Results in the place of what other workgroups still read.
+    (tables(kv=P, cu=P + 2 ** 16, slots=P + 2 ** 17, table=P + 2 ** 18), "overlaps an input"),
+    (tables(kv=P + 2 ** 15, cu=P + 2 ** 16, slots=P + 2 ** 17, table=P + 8), "overlaps an input"),
+]
+
+
 @pytest.mark.parametrize("call,msg", REFUSED, ids=lambda x: x if isinstance(x, str) else None)
 def test_refused(abi, call, msg):
     name, args = call
