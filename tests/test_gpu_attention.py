@@ -410,3 +410,217 @@ def test_paged_equals_packed(dev):
     diff = (paged.float() - packed.float()).abs()
     # Both within their bound of the same value: together twice a step of bf16 of the terms' size.
     assert float(diff.max()) <= 4 * 2.0 ** -8 * float(v.float().abs().max())
+
+
+# ---------------------------------------------------------------------------
+# Many requests, strides, sizes at random.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("R", (64, 65, 129, 256, 257, 700))
+def test_many_requests(dev, R):
+    """Past 64 requests a wave looks after four each, past 256 the keys are not split."""
+    g = torch.Generator().manual_seed(R)
+
+    def ints(hi):
+        return torch.randint(0, hi, (R,), generator=g).tolist()
+    paged_case(dev, [1] * R, [c if r % 7 else 0 for r, c in enumerate(ints(90))], 16, 4, 2, 64, BF16,
+               True, seed=R)
+    new = [n if n < 4 else 0 for n in ints(7)]
+    new[R // 2], new[-1] = 70, 41
+    paged_case(dev, new, ints(50), 7, 6, 2, 64, FP16, True, seed=R + 1, pad=5)
+    lens = [n if n < 9 else 0 for n in ints(12)]
+    lens[3], lens[R - 2] = 150, 33
+    varlen_case(dev, lens, lens, 4, 1, 128, BF16, True, seed=R + 2, pad=3)
+
+
+def test_long_context_beside_many_short_ones(dev):
+    for R in (66, 258):
+        ctx = [3] * R
+        ctx[R - 1], ctx[10] = 4000, 1500
+        paged_case(dev, [1] * R, ctx, 16, 8, 1, 128, BF16, True, seed=70)
+        paged_case(dev, [1] * (R - 1) + [90], ctx, 16, 8, 1, 128, BF16, True, seed=71)
+
+
+def test_strides(dev):
+    """Head-major q and out, K and V of different strides, one key head seen as many."""
+    T, Hq, D = 150, 4, 128
+    cu, lens = [0, 100, 150], [100, 50]
+    q, k, v = (randn((T, Hq, D), BF16, 80 + i) for i in range(3))
+    reqs = [(cu[r], cu[r + 1], k[cu[r]:cu[r + 1]], v[cu[r]:cu[r + 1]],
+             seen_mask(lens[r], lens[r], True)) for r in range(2)]
+
+    def major(x):  # the same values, heads outermost
+        return x.transpose(0, 1).contiguous().to(dev).transpose(0, 1)
+    wide = torch.zeros(T, Hq, D + 24, dtype=BF16, device=dev)
+    wide[:, :, 8:D + 8] = v.to(dev)
+    out = major(torch.zeros(T, Hq, D, dtype=BF16))
+    got = jo.attention_varlen(major(q), k.to(dev), wide[:, :, 8:D + 8], i32(cu, dev), out=out)
+    assert got is out
+    check(got, q, reqs, D ** -0.5, BF16)
+    one = jo.attention_varlen(q.to(dev), k[:, :1].to(dev).expand(T, 2, D),
+                              major(v[:, :1]).expand(T, 2, D), i32(cu, dev))
+    reqs = [(a, b, k[a:b, :1], v[a:b, :1], s) for a, b, _, _, s in reqs]
+    check(one, q, reqs, D ** -0.5, BF16)
+
+
+def test_paged_out_keeps_other_rows(dev):
+    q, pk, pv, table, cu, kv = step_inputs(dev, 4)
+    want = jo.attention_paged(q, pk, pv, table, cu, kv)
+    more = torch.cat((q, q[:20]))
+    out = torch.full_like(more, 5.0)
+    assert jo.attention_paged(more, pk, pv, table, cu, kv, out=out) is out
+    assert torch.equal(out[:q.shape[0]], want) and bool((out[q.shape[0]:] == 5).all())
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_sizes_at_random(dev, seed):
+    g = torch.Generator().manual_seed(1000 + seed)
+
+    def pick(*of):
+        return of[int(torch.randint(0, len(of), (1,), generator=g))]
+
+    def ints(n, hi):
+        return torch.randint(0, hi + 1, (n,), generator=g).tolist()
+    R, Hkv, G = pick(1, 2, 3, 5, 17), pick(1, 2, 3), pick(1, 2, 3, 5, 8)
+    D, dtype, causal = pick(64, 128, 256), pick(BF16, FP16), pick(True, True, False)
+    top = pick(1, 3, 20, 150)
+    new, ctx = ints(R, top), ints(R, pick(0, 5, 90, 1500))
+    paged_case(dev, new, ctx, pick(1, 5, 16, 24, 52, 64, 100, 128), Hkv * G, Hkv, D, dtype, causal,
+               seed=2000 + seed, pad=pick(0, 3), head_major=pick(True, False))
+    varlen_case(dev, new, pick(new, ints(R, 300)), Hkv * G, Hkv, D, dtype, causal, seed=3000 + seed,
+                pad=pick(0, 3))
+
+
+# ---------------------------------------------------------------------------
+# The C entry points, and what is refused.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("short", (None, 16, -16))
+def test_workspace_of_the_c_entry_point(dev, abi, short):
+    """None, or less than the plan's: the keys are not split, and the result is as good."""
+    q, pk, pv, table, cu, kv = step_inputs(dev, 5, new=(1, 1), ctx=(3000, 40))
+    T, Hq, D = q.shape
+    N, P, Hkv, _ = pk.shape
+    need = abi.lib().jo_attention_workspace_bytes(T, 2, Hq, Hkv, D, table.shape[1] * P)
+    assert need > 16
+    size = 0 if short is None else short % need if short > 0 else need + short
+    ws = torch.empty(max(size, 16) + 64, dtype=torch.uint8, device=dev).fill_(7)
+    out = torch.empty_like(q)
+    st = abi.lib().jo_attention_paged(
+        q.data_ptr(), pk.data_ptr(), pv.data_ptr(), out.data_ptr(), T, 2, Hq, Hkv, D, N, P,
+        Hq * D, D, P * Hkv * D, Hkv * D, D, P * Hkv * D, Hkv * D, D, Hq * D, D, table.data_ptr(),
+        table.shape[1], table.shape[1], cu.data_ptr(), kv.data_ptr(), D ** -0.5, 1, 1, 2,
+        ws.data_ptr() if short is not None else None, size,
+        torch.cuda.current_stream(dev).cuda_stream)
+    assert st == abi.JO_OK, abi.last_error()
+    reqs = []
+    for r in range(2):
+        m = int(kv[r])
+        k, v = (x.cpu()[table[r].cpu().clamp(min=0).long()].flatten(0, 1)[:m] for x in (pk, pv))
+        reqs.append((r, r + 1, k, v, seen_mask(1, m, True)))
+    check(out, q.cpu(), reqs, D ** -0.5, BF16)
+    assert bool((ws == 7).all())
+
+
+def test_refused_tensors(dev):
+    q, pk, pv, table, cu, kv = step_inputs(dev, 6)
+    k = torch.zeros(q.shape[0], 2, 128, dtype=BF16, device=dev)
+    vl, pg = jo.attention_varlen, jo.attention_paged
+
+    def no(msg, call, *a, **kw):
+        with pytest.raises((RuntimeError, ValueError, TypeError), match=msg):
+            call(*a, **kw)
+    no("bf16 or fp16", vl, q.float(), k.float(), k.float(), cu)
+    no("q's dtype", vl, q, k.half(), k, cu)
+    no("q's dtype", vl, q, k, k, cu, out=torch.empty_like(q).half())
+    no("must be on", vl, q, k.cpu(), k, cu)
+    no("cu_q", vl, q, k, k, cu.cpu())
+    no("cu_q", vl, q, k, k, cu.long())
+    no("cu_k", vl, q, k, k, cu, cu[:-1])
+    no("kv_lens", pg, q, pk, pv, table, cu, kv[:-1])
+    no("kv_lens", pg, q, pk, pv, table, cu, kv.long())
+    no("block_table", pg, q, pk, pv, table.long(), cu, kv)
+    no("block_table", pg, q, pk, pv, table.t(), cu, kv)
+    no("q's tokens", vl, q, k[:5], k[:5], cu)
+    no("key tensor's shape", vl, q, k, k[:, :1], cu)
+    no("key tensor's shape", pg, q, pk, pv[:3], table, cu, kv)
+    no("multiple of the key heads", vl, q[:, :7], k, k, cu)
+    no("head_dim", vl, q[:, :, :96], k[:, :, :96], k[:, :, :96], cu)
+    no("tokens, heads, head_dim", vl, q[0], k, k, cu)
+    no("pages, page_size", pg, q, k, k, table, cu, kv)
+    no("contiguous head_dim", vl, q[:, :, ::2], k[:, :, :64], k[:, :, :64], cu)
+    no("multiples of 8", vl, torch.zeros(q.shape[0], 8, 132, dtype=BF16, device=dev)[:, :, :128], k, k, cu)
+    flat = torch.zeros(q.numel() + 8, dtype=BF16, device=dev)
+    no("16-byte aligned", vl, flat[4:-4].view(q.shape), k, k, cu)
+    no("out must have q's shape", vl, q, k, k, cu, out=torch.empty_like(q)[:-1])
+    no("overlap an input", vl, q, k, k, cu, out=q)
+    no("overlap an input", vl, q, k, k, cu, out=q.view(-1)[:].view(q.shape))
+    no("must not overlap", vl, q, k, k, cu, out=torch.empty_like(q[:1]).expand_as(q))
+    rows = torch.empty(q.shape[0] * 256 + 1024, dtype=BF16, device=dev)
+    no("must not overlap", vl, q, k, k, cu, out=rows.as_strided(q.shape, (256, 128, 1)))
+    no("scale", vl, q, k, k, cu, scale=0.0)
+    no("scale", vl, q, k, k, cu, scale=math.nan)
+
+
+def test_refused_tables_and_commits(dev):
+    ctx, new, n = i32([3, 9], dev), i32([1, 1], dev), i32([4], dev)
+    table, free = torch.full((2, 4), -1, dtype=torch.int32, device=dev), i32(list(range(9)), dev)
+
+    def no(msg, call, *a, **kw):
+        with pytest.raises((RuntimeError, ValueError, TypeError), match=msg):
+            call(*a, **kw)
+    no("same length", jo.paged_tables, ctx, new[:1], table, free, n, 4, 9, 8)
+    no("new_lens", jo.paged_tables, ctx, new.long(), table, free, n, 4, 9, 8)
+    no("num_free", jo.paged_tables, ctx, new, table, free, ctx, 4, 9, 8)
+    no("block_table", jo.paged_tables, ctx, new, table[:1], free, n, 4, 9, 8)
+    no("block_table", jo.paged_tables, ctx, new, table.t(), free, n, 4, 9, 8)
+    no("free_pages", jo.paged_tables, ctx, new, table, free.cpu(), n, 4, 9, 8)
+    no("max_tokens", jo.paged_tables, ctx, new, table, free, n, 4, 9, -1)
+    no("page_size", jo.paged_tables, ctx, new, table, free, n, 0, 9, 8)
+    no("table stride", jo.paged_tables, ctx, new, table[:1].expand(2, 4), free, n, 4, 9, 8)
+    src, pages = (torch.zeros(s, dtype=BF16, device=dev) for s in ((2, 2, 64), (3, 4, 2, 64)))
+    slots, cos = torch.zeros(2, dtype=torch.int64, device=dev), torch.ones(2, 64, device=dev)
+    c = jo.kv_commit_rope_paged
+    no("slots", c, src, pages, slots.int())
+    no("slots", c, src, pages, slots[:1])
+    no("dtype", c, src, pages.half(), slots)
+    no("bf16 or fp16", c, src.float(), pages.float(), slots)
+    no("src_k's heads", c, src, pages[:, :, :1], slots)
+    no("go together", c, src, pages, slots, cos)
+    no("go together", c, src, pages, slots, src_v=src)
+    no("cos and sin", c, src, pages, slots, cos, cos[:1])
+    no("contiguous heads", c, src, pages.transpose(1, 2).contiguous().transpose(1, 2), slots)
+
+
+def test_two_streams_at_once(dev):
+    """Calls of two streams side by side: each has a workspace of its own."""
+    a, b = step_inputs(dev, 7), step_inputs(dev, 8, new=(1, 1, 1), ctx=(6000, 100, 9))
+    want = [jo.attention_paged(*x) for x in (a, b)]
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(dev))
+    for _ in range(8):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(jo.attention_paged(*x))
+    torch.cuda.synchronize(dev)
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_ops_keep_to_their_schemas(dev):
+    """What the schemas and the shape functions say of results, changed inputs and aliases."""
+    q, pk, pv, table, cu, kv = step_inputs(dev, 9)
+    tests = ("test_schema", "test_faketensor")
+    ops = torch.ops.joyomni_ops
+    k = torch.zeros(q.shape[0], 2, 128, dtype=BF16, device=dev)
+    torch.library.opcheck(ops.attention_varlen.default, (q, k, k, cu, None, None, True), test_utils=tests)
+    torch.library.opcheck(ops.attention_paged.default, (q, pk, pv, table, cu, kv, None, True),
+                          test_utils=tests)
+    torch.library.opcheck(ops.attention_paged_out.default,
+                          (q, pk, pv, table, cu, kv, None, True, torch.empty_like(q)), test_utils=tests)
+    torch.library.opcheck(ops.paged_tables.default,
+                          (kv, torch.ones_like(kv), table, torch.arange(9, device=dev, dtype=torch.int32),
+                           i32([9], dev), 16, pk.shape[0], 8), test_utils=tests)
+    torch.library.opcheck(ops.kv_commit_rope_paged.default,
+                          (k, k, pk, pv, torch.arange(k.shape[0], device=dev), None, None),
+                          test_utils=tests)
