@@ -604,7 +604,8 @@ int jo_attention_paged(const void* q, const void* pages_k, const void* pages_v, 
  * kv_capacity is kv_tokens, or table_width * page_size. A host-side
  * computation; a few hundred MB at most. */
 int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests, int64_t q_heads,
-                                     int64_t kv_heads, int64_t head_dim, int64_t kv_capacity);
+                                     int64_t kv_heads, int64_t head_dim, int64_t kv_capacity,
+                                     int causal);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -11,6 +11,9 @@
 namespace jo {
 namespace {
 
+// A lambda that is never a call: what it captures stays in registers.
+#define JO_INLINE __attribute__((always_inline))
+
 struct AttnArgs {
   const void* q;
   const void* k;
@@ -34,6 +37,8 @@ struct AttnArgs {
   uint32_t items;                    // work items launched, a key head each
   uint32_t split_target;             // 0: keys are not split
   FastDiv fd_target;                 // its division
+  uint32_t tail_splits, tail_most;   // the last round's splits (1: none), and of how many tiles
+  FastDiv fd_round;                  // division by a round's tiles
   float* ws;                         // partial results of split items
 };
 
@@ -173,6 +178,10 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, int r, const Reque
 //   chunk = max(kMinChunk, floor(cost / split_target) + 1),
 //   splits = ceil(key blocks / chunk), items = tiles x splits, in request order,
 // so there are at most tiles + split_target items, which is what is launched.
+// Or (tail_splits > 1) all tiles of the rounds that fill the GPU are whole, and
+// only those of the last round, `tail` of them, are split:
+//   tail = tiles mod round, if that is no more than tail_most (else nothing is),
+//   splits = min(tail_splits, key blocks / kMinChunk), for the last `tail` tiles.
 // With more requests keys are not split, and request r's tiles begin at index
 // floor(cu_q[r] x group / ROWS) + r, which leaves each room for its tiles.
 // ---------------------------------------------------------------------------
@@ -189,8 +198,8 @@ struct Item {
   int tile;            // rows [tile * ROWS, ...) of the request
   int split, splits;   // this range of the keys, and how many there are
   int chunk;           // key blocks a range
-  int index;           // of the item (a partial result's place); in the joining kernel: of the
-                       // tile's first item
+  int index;           // a partial result's place: items in order, from the first that is split
+                       // (in the joining kernel: of the tile's first)
 };
 
 // Inclusive prefix sum over the wave (saturating), with DPP: shifts within rows
@@ -238,14 +247,39 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
     chunk = max(static_cast<uint32_t>(kMinChunk), fdiv(total, a.fd_target) + 1);
     if (total == UINT32_MAX) chunk = kNoSplit;  // a saturated total says too little
   }
-  uint32_t splits[E], items = 0, units = 0;
+  uint32_t splits[E], whole[E], items = 0, units = 0;
+  uint32_t full = 0;  // tiles of the rounds before the last, which is split
+  if (a.tail_splits > 1) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine += tiles[e];
+    const uint32_t end = wave_scan(mine);
+    const uint32_t total = __builtin_amdgcn_readlane(end, kWave - 1);
+    const uint32_t tail = total - fdiv(total, a.fd_round) * a.fd_round.d;
+    full = tail <= a.tail_most ? total - tail : total;
+    uint32_t at = end - mine;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      whole[e] = min(tiles[e], full - min(full, at));
+      at += tiles[e];
+    }
+  }
+  auto units_of = [&](int e) JO_INLINE {
+    return TILES ? (splits[e] > 1 ? tiles[e] - whole[e] : 0)
+                 : whole[e] + (tiles[e] - whole[e]) * splits[e];
+  };
   // (One division of 32 bits a request; in fp32 first, blocks and chunk being
   // below 2^24 in any pool that exists, would not hold for all inputs.)
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    splits[e] = blocks[e] <= chunk ? 1u : (blocks[e] - 1) / chunk + 1;
-    items += tiles[e] * splits[e];
-    units += TILES ? (splits[e] > 1 ? tiles[e] : 0) : tiles[e] * splits[e];
+    if (a.tail_splits > 1) {
+      splits[e] = max(1u, min(a.tail_splits, blocks[e] / kMinChunk));
+    } else {
+      splits[e] = blocks[e] <= chunk ? 1u : (blocks[e] - 1) / chunk + 1;
+      whole[e] = 0;
+    }
+    items += whole[e] + (tiles[e] - whole[e]) * splits[e];
+    units += units_of(e);
   }
   const uint32_t unit_end = wave_scan(units);
   const uint32_t item_end = TILES ? wave_scan(items) : unit_end;
@@ -254,18 +288,17 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
   const int owner = __builtin_ctzll(past);
   // In the owner lane: which of its requests, and the index within it.
   uint32_t local = id - (unit_end - units), first = item_end - items;
-  uint32_t e_found = 0, n_splits = splits[0], n_tiles = tiles[0], n_blocks = blocks[0];
+  uint32_t e_found = 0, n_splits = splits[0], n_tiles = tiles[0], n_blocks = blocks[0],
+           n_whole = whole[0];
   Request y = x[0];
-  auto units_of = [&](int e) {
-    return TILES ? (splits[e] > 1 ? tiles[e] : 0) : tiles[e] * splits[e];
-  };
   bool found = local < units_of(0);
 #pragma unroll
   for (int e = 1; e < E; ++e) {
     if (!found) {
       local -= units_of(e - 1);
-      first += tiles[e - 1] * splits[e - 1];
+      first += whole[e - 1] + (tiles[e - 1] - whole[e - 1]) * splits[e - 1];
       e_found = e, n_splits = splits[e], n_tiles = tiles[e], n_blocks = blocks[e];
+      n_whole = whole[e];
       y = x[e];
       found = local < units_of(e);
     }
@@ -281,14 +314,17 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
   it.x = Request{of_owner(y.q0), of_owner(y.nq), of_owner(y.k0), of_owner(y.keys),
                  of_owner(y.first_pos)};
   it.r = owner * E + of_owner(e_found);
-  it.splits = n_splits;
+  n_whole = of_owner(n_whole);
+  const bool one = n_splits == 1 || (!TILES && local < n_whole);
+  it.splits = one ? 1 : n_splits;
   // The ranges of a request are of one length, to a block.
-  it.chunk = n_splits == 1 ? kNoSplit : (n_blocks - 1) / n_splits + 1;
-  const uint32_t t = TILES || n_splits == 1 ? local : local / n_splits;
-  it.split = TILES ? 0 : local - t * n_splits;
+  it.chunk = one ? kNoSplit : (n_blocks - 1) / n_splits + 1;
+  const uint32_t rest = TILES ? local : local - n_whole;
+  const uint32_t t = one ? local : n_whole + (TILES ? rest : rest / n_splits);
+  it.split = one || TILES ? 0 : rest - (t - n_whole) * n_splits;
   // The last tile first: with a causal mask it sees the most keys.
   it.tile = n_tiles - 1 - t;
-  it.index = TILES ? first + t * n_splits : id;
+  it.index = (TILES ? first + n_whole + rest * n_splits : id) - full;
   return it;
 }
 
@@ -398,8 +434,6 @@ __device__ __forceinline__ u32x4 lds_read_tr(uint32_t addr0, uint32_t addr1) {
 // counter to 0.
 #define JO_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(0x0F70 | ((n) & 15) | (((n) >> 4) << 14))
 #define JO_WAIT_LDS0() __builtin_amdgcn_s_waitcnt(0xC07F)
-// A lambda that is never a call: what it captures stays in registers.
-#define JO_INLINE __attribute__((always_inline))
 // Keeps memory accesses on their side of it (the compiler does not know what the
 // waits above wait for).
 #define JO_KEEP_ORDER() asm volatile("" ::: "memory")
@@ -1201,6 +1235,7 @@ struct AttnPlan {
   bool few;             // attn_few_kernel
   int64_t tiles;        // at most so many
   int64_t split_target;
+  int64_t tail_splits, tail_most, round;
   int64_t items;
   int64_t ws_bytes;
 };
@@ -1213,8 +1248,8 @@ constexpr int64_t kComputeUnits = 256;
 constexpr int kFewJoin = 4, kTileJoin = 1, kTileEach = 2;  // threads that share an element's splits
 
 AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
-                        int64_t head_dim, int64_t kv_capacity) {
-  AttnPlan p;
+                        int64_t head_dim, int64_t kv_capacity, bool causal) {
+  AttnPlan p{};
   const int64_t group = q_heads / kv_heads;
   const int64_t all_rows = q_tokens * group;
   p.few = all_rows <= 16 * requests;
@@ -1239,7 +1274,36 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
     p.split_target = p.tiles <= round / 2 ? round - p.tiles : p.few ? 2 * round : round;
   const int64_t most = p.tiles * (blocks / kMinChunk + 1);
   p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;
-  p.ws_bytes = p.split_target == 0 ? 0 : p.items * kv_heads * rows * (head_dim + 2) * 4;
+  // Tiles that see all keys take equally long, and a last round of a few leaves
+  // most of the GPU idle: its tiles are split where that is worth the partial
+  // results' way to memory and back. Times in key blocks of a tile: one a CU is
+  // 1 us, joining 5 us and 6.5 us a partial result and CU. (Two frames of 1560
+  // tokens over three cached ones and themselves, 32 heads: 25 tiles a head, 16 a
+  // round; not split 555 us, the last 9 in two 539, three 531, four, as chosen
+  // here, 528, six 539, eight 548.)
+  int64_t places = p.split_target == 0 ? 0 : p.items;
+  p.round = round;
+  p.tail_splits = 1;
+  if (!p.few && !causal && p.split_target == 0 && requests > 0 && requests <= kPlanRequests &&
+      p.tiles > round) {
+    // Requests taken to be alike.
+    const int64_t each = (q_tokens / requests * group + rows - 1) / rows;
+    const int64_t tail = requests * each % round;
+    auto time = [&](int64_t s) {  // in blocks
+      const int64_t n = tail * kv_heads * s;
+      const int64_t steps = (n + kComputeUnits - 1) / kComputeUnits;
+      return static_cast<double>(steps) * static_cast<double>(blocks) / static_cast<double>(s) +
+             (s == 1 ? 0. : 5. + 6.5 * static_cast<double>(n) / kComputeUnits);
+    };
+    for (int64_t s = 2; s <= 8 && s * kMinChunk <= blocks; ++s)
+      if (time(s) < time(p.tail_splits)) p.tail_splits = s;
+    if (p.tail_splits > 1) {
+      p.tail_most = tail;
+      p.items += tail * (p.tail_splits - 1);
+      places = tail * p.tail_splits;
+    }
+  }
+  p.ws_bytes = places * kv_heads * rows * (head_dim + 2) * 4;
   return p;
 }
 
@@ -1247,13 +1311,17 @@ template <class Tag, int D, bool PAGED>
 int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes,
                      hipStream_t stream) {
   const char* op = PAGED ? "attention_paged" : "attention_varlen";
-  AttnPlan p = plan_attention(a.q_tokens, a.requests, a.q_heads, a.kv_heads, D, kv_capacity);
+  AttnPlan p = plan_attention(a.q_tokens, a.requests, a.q_heads, a.kv_heads, D, kv_capacity, a.causal);
   if (p.ws_bytes > 0 && ws_bytes < p.ws_bytes) {  // none, or one for another call: no splits
     p.split_target = 0;
+    p.tail_splits = 1;
     p.items = p.tiles;
   }
   a.split_target = static_cast<uint32_t>(p.split_target);
   a.fd_target = make_fastdiv(a.split_target);
+  a.tail_splits = static_cast<uint32_t>(p.tail_splits);
+  a.tail_most = static_cast<uint32_t>(p.tail_most);
+  a.fd_round = make_fastdiv(static_cast<uint32_t>(p.round));
   a.items = static_cast<uint32_t>(p.items);
   a.ws = static_cast<float*>(ws);
   // Workgroups that clear the rows of no request, 64 KB each if they are all.
@@ -1273,10 +1341,12 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
   else
     hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages>), grid, dim3(kBlock), 0, stream, a);
   int st = launch_status(op);
-  if (st != JO_OK || p.split_target == 0) return st;
-  // Tiles that are split: no more than split_target, since each has more key
-  // blocks than a chunk.
-  const int64_t split_tiles = p.tiles < p.split_target ? p.tiles : p.split_target;
+  if (st != JO_OK || (p.split_target == 0 && p.tail_splits == 1)) return st;
+  // Tiles that are split: the tail's, or no more than split_target, since each has
+  // more key blocks than a chunk.
+  const int64_t split_tiles = p.tail_splits > 1 ? p.tail_most
+                              : p.tiles < p.split_target ? p.tiles
+                                                         : p.split_target;
   const int64_t joins = split_tiles * a.kv_heads * (p.few ? 16 : kTileRows) * (D / 4) *
                         (p.few ? kFewJoin : kTileJoin) / kBlock / (p.few ? 1 : kTileEach);
   JO_REQUIRE(joins <= INT32_MAX / 512, "%s: shape too large", op);
@@ -1452,9 +1522,11 @@ extern "C" int jo_attention_paged(const void* q, const void* pages_k, const void
 
 extern "C" int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests,
                                                 int64_t q_heads, int64_t kv_heads,
-                                                int64_t head_dim, int64_t kv_capacity) {
+                                                int64_t head_dim, int64_t kv_capacity,
+                                                int causal) {
   if (q_tokens <= 0 || requests < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
       head_dim <= 0 || kv_capacity < 0)
     return 0;
-  return plan_attention(q_tokens, requests, q_heads, kv_heads, head_dim, kv_capacity).ws_bytes;
+  return plan_attention(q_tokens, requests, q_heads, kv_heads, head_dim, kv_capacity, causal != 0)
+      .ws_bytes;
 }

@@ -1241,8 +1241,8 @@ void attn_no_overlap(const torch::Tensor& out, std::initializer_list<const torch
   }
 }
 
-void attn_workspace(AttnCall& c, const torch::Tensor& q, int64_t kv_capacity) {
-  c.ws_bytes = jo_attention_workspace_bytes(c.T, c.R, c.Hq, c.Hkv, c.D, kv_capacity);
+void attn_workspace(AttnCall& c, const torch::Tensor& q, int64_t kv_capacity, bool causal) {
+  c.ws_bytes = jo_attention_workspace_bytes(c.T, c.R, c.Hq, c.Hkv, c.D, kv_capacity, causal);
   if (c.ws_bytes > 0) c.ws = torch::empty({c.ws_bytes}, q.options().dtype(torch::kUInt8));
 }
 
@@ -1259,7 +1259,7 @@ void run_varlen(const torch::Tensor& q, const torch::Tensor& k, const torch::Ten
   }
   if (q.numel() == 0) return;
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
-  attn_workspace(c, q, k.size(0));
+  attn_workspace(c, q, k.size(0), causal);
   check_status(jo_attention_varlen(
                    q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), c.T, k.size(0), c.R,
                    c.Hq, c.Hkv, c.D, c.q.ts, c.q.hs, c.k.ts, c.k.hs, c.v.ts, c.v.hs, c.o.ts,
@@ -1282,7 +1282,7 @@ void run_paged(const torch::Tensor& q, const torch::Tensor& pages_k, const torch
   TORCH_CHECK(kv_lens.numel() == c.R, "kv_lens must be [requests]");
   if (q.numel() == 0) return;
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
-  attn_workspace(c, q, W * P);
+  attn_workspace(c, q, W * P, causal);
   check_status(jo_attention_paged(
                    q.data_ptr(), pages_k.data_ptr(), pages_v.data_ptr(), out.data_ptr(), c.T, c.R,
                    c.Hq, c.Hkv, c.D, N, P, c.q.ts, c.q.hs, c.k.ps, c.k.ts, c.k.hs, c.v.ps, c.v.ts,

@@ -104,7 +104,7 @@ SIGNATURES: dict[str, list] = {
         _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
         _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _F, c_int, c_int, c_int, _P, _I64,
         _P],
-    "jo_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64],
+    "jo_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64, c_int],
 }
 
 _lib = None

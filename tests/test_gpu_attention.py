@@ -499,7 +499,7 @@ def test_workspace_of_the_c_entry_point(dev, abi, short):
     q, pk, pv, table, cu, kv = step_inputs(dev, 5, new=(1, 1), ctx=(3000, 40))
     T, Hq, D = q.shape
     N, P, Hkv, _ = pk.shape
-    need = abi.lib().jo_attention_workspace_bytes(T, 2, Hq, Hkv, D, table.shape[1] * P)
+    need = abi.lib().jo_attention_workspace_bytes(T, 2, Hq, Hkv, D, table.shape[1] * P, 1)
     assert need > 16
     size = 0 if short is None else short % need if short > 0 else need + short
     ws = torch.empty(max(size, 16) + 64, dtype=torch.uint8, device=dev).fill_(7)
@@ -624,3 +624,22 @@ def test_ops_keep_to_their_schemas(dev):
     torch.library.opcheck(ops.kv_commit_rope_paged.default,
                           (k, k, pk, pv, torch.arange(k.shape[0], device=dev), None, None),
                           test_utils=tests)
+
+
+@pytest.mark.parametrize("lq,lk", (([3100], [5000]), ([1100, 1090, 1100], [4200, 4200, 4100]),
+                                   ([2500, 400, 400], [4300, 90, 4200]), ([2100, 0, 1], [4200, 0, 4200])),
+                         ids=("one", "alike", "not-alike", "nearly-one"))
+@pytest.mark.parametrize("D", (64, 128))
+def test_last_round_split(dev, D, lq, lk):
+    """Tokens that see every key, more tiles than the GPU runs at once and not a multiple: the last
+    round's tiles have their keys split. A few heads against the definition."""
+    H, heads = 32, [0, 17, 31]
+    q = randn((sum(lq), H, D), BF16, 90, 1.3)
+    k, v = (randn((sum(lk), H, D), BF16, 91 + i, 1.3 - 0.3 * i) for i in range(2))
+    cq, ck = cu_of(lq), cu_of(lk)
+    got = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32(cq, dev), i32(ck, dev), causal=False)
+    reqs = [(cq[r], cq[r + 1], k[ck[r]:ck[r + 1], heads], v[ck[r]:ck[r + 1], heads],
+             seen_mask(lq[r], lk[r], False)) for r in range(len(lq))]
+    check(got[:, heads], q[:, heads], reqs, D ** -0.5, BF16)
+    again = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32(cq, dev), i32(ck, dev), causal=False)
+    assert torch.equal(got, again)
