@@ -662,6 +662,21 @@ __device__ __forceinline__ void store_tile(const AttnArgs a, const Item& it, int
 // consecutive keys of one column of V at a time, just those.
 // K and V blocks go straight from global memory to LDS, one block ahead of
 // their use; one barrier a block.
+//
+// Per block and wave (D = 128) the products take 1024 cycles of a matrix unit,
+// reading their operands 256 cycles of the CU's LDS (so eight waves' reads take as
+// long as all four matrix units do: 32 rows a wave is the least that works, and
+// 64 rows a wave leave one wave a SIMD: 761 against 1060 TFLOP/s), the weights
+// about 1000 cycles of the vector unit, half of them 32 exponentials. Two
+// workgroups share a CU, so one's weights run beside the other's products.
+// Measured: a prompt of 16384 tokens, 32 heads over 8 of 128, causal, 2.0 to 2.3
+// ms by the card's clock (1.10 to 0.96 PFLOP/s; a plain product of 8192^3 reaches
+// 1.21), matrix units busy 61% of the cycles at 1.5 GHz, no bank conflicts: power
+// and the LDS bound it. 16384 tokens of 32 over 16 heads of 64: 0.87 PFLOP/s (the
+// exponentials); 12000 of 16 over 4 of 256: 0.85 (one workgroup a CU, 128 KB of
+// LDS). Dropped: eight waves in two groups a phase apart (1.03 to 1.05), blocks
+// of 32 keys with the weights a block behind (1.06, short prompts slower), raised
+// wave priority (level), heads grouped by XCD (level; D = 256 slower).
 // ---------------------------------------------------------------------------
 template <class Tag, int D, Keys KEYS>
 __global__ __launch_bounds__(kBlock, D <= 128 ? 2 : 1) void attn_tiles_kernel(const AttnArgs a) {
@@ -926,6 +941,14 @@ __global__ __launch_bounds__(kBlock, D <= 128 ? 2 : 1) void attn_tiles_kernel(co
 // at a time each, with 16x16x32 products in the same transposed form. Every
 // wave loads its own keys into its own part of LDS, a block ahead, and waits for
 // no other wave until the waves' results are joined at the end.
+//
+// Bound by reading the keys once: 64 requests of 100 to 16384 keys, 8 key heads
+// of 128, 148 us (5.0 TB/s; a large copy moves 5.15), two of 100000 keys 95 us
+// (5.3), 256 of 500 to 2000 211 us (5.3); four of 300 to 2000 keys 11 us, of
+// which the joining kernel takes 3 and a launch 4: latency. Measured level: four
+// or two waves a workgroup (the latter 4 to 8% slower in full batches), page ids
+// of 32 blocks at a time. Items that share an XCD by request instead of by key
+// head: 64 requests 148 -> 203 us.
 // ---------------------------------------------------------------------------
 template <int D>
 struct FewShape {

