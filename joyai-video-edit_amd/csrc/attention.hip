@@ -1293,7 +1293,8 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   // over long contexts among chunks), one tile can outlast all others.
   const bool full = !p.few && kv_capacity <= 4 * q_tokens &&
                     (requests == 1 ? p.tiles > round : 4 * p.tiles >= 7 * round);
-  if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && p.tiles < 8 * round && !full)
+  if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && p.tiles < 8 * round &&
+      kv_heads <= slots && !full)
     p.split_target = p.tiles <= round / 2 ? round - p.tiles : p.few ? 2 * round : round;
   const int64_t most = p.tiles * (blocks / kMinChunk + 1);
   p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;

@@ -643,3 +643,42 @@ def test_last_round_split(dev, D, lq, lk):
     check(got[:, heads], q[:, heads], reqs, D ** -0.5, BF16)
     again = jo.attention_varlen(q.to(dev), k.to(dev), v.to(dev), i32(cq, dev), i32(ck, dev), causal=False)
     assert torch.equal(got, again)
+
+
+def test_compiled_without_a_graph_break(dev):
+    """A step's four calls, traced: the block table and the pages are changed in place."""
+    g = torch.Generator().manual_seed(5)
+    P, N, D, T = 16, 20, 64, 8
+
+    def step(q, k, v, pk, pv, ctx, new, table, free, n):
+        cu, kv, slots, left = jo.paged_tables(ctx, new, table, free, n, P, N, T)
+        jo.kv_commit_rope_paged(k, pk, slots, src_v=v, pages_v=pv)
+        o = jo.attention_paged(q, pk, pv, table, cu, kv)
+        into = torch.zeros_like(o)
+        jo.attention_varlen(q, k, v, cu, out=into)
+        return o, into, left, jo.attention_varlen(q, k, v, cu, causal=False)
+
+    def inputs():
+        g.manual_seed(5)
+        rnd = lambda *s: torch.randn(*s, generator=g).to(BF16).to(dev)  # noqa: E731
+        table = torch.full((2, 6), -1, dtype=torch.int32, device=dev)
+        table[0, :3] = i32([4, 9, 2], dev)
+        return [rnd(T, 4, D), rnd(T, 2, D), rnd(T, 2, D), rnd(N, P, 2, D), rnd(N, P, 2, D),
+                i32([40, 0], dev), i32([1, 5], dev), table, i32(list(range(10, 19)), dev), i32([9], dev)]
+    a, b = inputs(), inputs()
+    want = step(*a)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(*b)
+    for x, y in zip(list(got) + b, list(want) + a):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.filterwarnings("ignore::UserWarning")
+def test_forward_only(dev):
+    """No gradient reaches the inputs: the result warns when it is differentiated."""
+    q = randn((5, 2, 64), BF16, 1).to(dev).requires_grad_()
+    k = randn((5, 2, 64), BF16, 2).to(dev)
+    out = jo.attention_varlen(q, k, k, i32([0, 5], dev))
+    assert torch.equal(out.detach(), jo.attention_varlen(q.detach(), k, k, i32([0, 5], dev)))
+    with pytest.warns(UserWarning, match="autograd kernel was not registered"):
+        out.sum().backward()
+    assert q.grad is None
