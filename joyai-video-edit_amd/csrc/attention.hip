@@ -1285,17 +1285,32 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   const int64_t slots = kComputeUnits * (p.few ? (head_dim == 64 ? 2 : 1) : (head_dim <= 128 ? 2 : 1));
   const int64_t round = (slots + kv_heads - 1) / kv_heads;  // items of one round
   p.split_target = 0;
+  // How many tiles there are if the requests are alike.
+  const int64_t alike =
+      requests == 0 ? 0 : requests * ((q_tokens / requests * group + rows - 1) / rows);
   // Tiles of 128 rows that fill the GPU, with no more than a few keys a token:
   // their ranges would hardly be split, and the joining kernel's launch is saved
   // (four prompts of 1000 tokens, 2.0 rounds: 64.2 -> 59.5 us, eight of 200 to
-  // 3500, 2.3 rounds: 62.1 -> 59.3). One request's tiles are alike: they are split
-  // below one round only. Where keys may be many more than tokens (single tokens
+  // 3500, 2.3 rounds: 62.1 -> 59.3). One request's tiles are alike, all of them
+  // where every key is seen. Where keys may be many more than tokens (single tokens
   // over long contexts among chunks), one tile can outlast all others.
-  const bool full = !p.few && kv_capacity <= 4 * q_tokens &&
-                    (requests == 1 ? p.tiles > round : 4 * p.tiles >= 7 * round);
+  const bool full =
+      !p.few && kv_capacity <= 4 * q_tokens &&
+      (requests == 1 ? (causal ? 1 : 2) * alike > round : 4 * p.tiles >= 7 * round);
   if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && p.tiles < 8 * round &&
-      kv_heads <= slots && !full)
-    p.split_target = p.tiles <= round / 2 ? round - p.tiles : p.few ? 2 * round : round;
+      kv_heads <= slots && !full) {
+    // A split tile's last range is half full on average: split_target + tiles / 2
+    // items come of it, and are meant to fill rounds: one where tiles are few (a
+    // little under it: unequal requests have more tiles; 32 requests of 16 tokens
+    // 52.9 us, with round - tiles 57.3, round - tiles / 2 51.2, but 10 of chunks and
+    // single tokens 108.7, 108.3, 110.2), else two or, of single tokens, up to three
+    // (24 single tokens 83.2 us with 1.5 rounds, 94 with one, 87 with two; 64 of them
+    // 148 with two rounds, 160 with 1.5, 168 with one).
+    if (2 * alike <= round)
+      p.split_target = round - 3 * alike / 4;
+    else
+      p.split_target = !p.few ? round : alike <= round ? 3 * round / 2 : 2 * round;
+  }
   const int64_t most = p.tiles * (blocks / kMinChunk + 1);
   p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;
   // Tiles that see all keys take equally long, and a last round of a few leaves
@@ -1309,10 +1324,8 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   p.round = round;
   p.tail_splits = 1;
   if (!p.few && !causal && p.split_target == 0 && requests > 0 && requests <= kPlanRequests &&
-      p.tiles > round) {
-    // Requests taken to be alike.
-    const int64_t each = (q_tokens / requests * group + rows - 1) / rows;
-    const int64_t tail = requests * each % round;
+      (requests == 1 || p.tiles > round)) {
+    const int64_t tail = alike % round;
     auto time = [&](int64_t s) {  // in blocks
       const int64_t n = tail * kv_heads * s;
       const int64_t steps = (n + kComputeUnits - 1) / kComputeUnits;
