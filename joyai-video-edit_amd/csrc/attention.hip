@@ -178,6 +178,12 @@ __device__ __forceinline__ void attend_row(const AttnArgs& a, int r, const Reque
 //   chunk = max(kMinChunk, floor(cost / split_target) + 1),
 //   splits = ceil(key blocks / chunk), items = tiles x splits, in request order,
 // so there are at most tiles + split_target items, which is what is launched.
+// With up to 64 requests the longest items go first, in 16 levels of length: a
+// long one that starts last is what all others wait for (eight prompts of 200 to
+// 3500 tokens 57.6 -> 49.3 us, 20 requests of chunks and single tokens 93 -> 83, 64
+// single tokens 148 -> 141). An item's level and place in it come of one count of
+// the items in the levels before for every halving of 16, which costs a wave about
+// a microsecond and is left out where the order cannot matter.
 // Or (tail_splits > 1) all tiles of the rounds that fill the GPU are whole, and
 // only those of the last round, `tail` of them, are split:
 //   tail = tiles mod round, if that is no more than tail_most (else nothing is),
@@ -198,8 +204,8 @@ struct Item {
   int tile;            // rows [tile * ROWS, ...) of the request
   int split, splits;   // this range of the keys, and how many there are
   int chunk;           // key blocks a range
-  int index;           // a partial result's place: items in order, from the first that is split
-                       // (in the joining kernel: of the tile's first)
+  int index;           // a partial result's place: items in request order, from the first that is
+                       // split (in the joining kernel: of the tile's first)
 };
 
 // Inclusive prefix sum over the wave (saturating), with DPP: shifts within rows
@@ -217,6 +223,23 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   JO_SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
 #undef JO_SCAN_STEP
   return v;
+}
+
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  return __builtin_amdgcn_readlane(wave_scan(v), kWave - 1);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define JO_MAX_STEP(ctrl, rows) \
+  v = max(v, static_cast<uint32_t>( \
+                 __builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xf, false)))
+  JO_MAX_STEP(0x111, 0xf);
+  JO_MAX_STEP(0x112, 0xf);
+  JO_MAX_STEP(0x114, 0xf);
+  JO_MAX_STEP(0x118, 0xf);
+  JO_MAX_STEP(0x142, 0xa);
+  JO_MAX_STEP(0x143, 0xc);
+#undef JO_MAX_STEP
+  return __builtin_amdgcn_readlane(v, kWave - 1);
 }
 
 constexpr uint32_t kNoSplit = 0x40000000u;  // beyond any number of key blocks
@@ -283,11 +306,45 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
   }
   const uint32_t unit_end = wave_scan(units);
   const uint32_t item_end = TILES ? wave_scan(items) : unit_end;
-  const uint64_t past = __ballot(unit_end > id);
+  // The lane whose request it is; in that lane: the index within the lane's.
+  uint64_t past = __ballot(unit_end > id);
+  uint32_t local = id - (unit_end - units);
+  if constexpr (E == 1 && !TILES) {
+    const uint32_t parts = (blocks[0] + splits[0] - 1) / splits[0];  // key blocks of a range
+    const uint32_t uncut = splits[0] > 1 ? whole[0] : items, cut = items - uncut;
+    const uint32_t longest = uncut > 0 ? blocks[0] : cut > 0 ? parts : 0;
+    const uint32_t top = wave_max(longest);
+    // Items in 16 levels by length: level l has those longer than (15 - l) / 16 of
+    // the longest. In order as they are: if all are of the first level, if they all
+    // run at once, or of one request.
+    const bool shorter = longest + top / 16 < top || (a.causal && uncut > 1);
+    if (a.items > a.fd_round.d && a.requests > 1 && __ballot(items > 0 && shorter) != 0) {
+      // Of uncut tiles with a causal mask each sees fewer keys than the one behind it,
+      // by a tile's share of a block.
+      const float step = a.causal ? static_cast<float>(a.group) * kKeyBlock / ROWS : 1e9f;
+      const float most = static_cast<float>(uncut);
+      auto up_to = [&](uint32_t level) JO_INLINE -> uint32_t {  // items of the levels below
+        const uint32_t x = (top >> 4) * (16 - level) + ((top & 15) * (16 - level) >> 4);
+        const float n = fminf(static_cast<float>(blocks[0] - x) * step, most);
+        const uint32_t u = x < blocks[0] ? min(uncut, static_cast<uint32_t>(n) + 1) : 0u;
+        const uint32_t c = x < parts ? cut : 0u;
+        return level == 0 ? 0u : level == 16 ? items : u + c;
+      };
+      uint32_t lo = 0, below = 0;
+#pragma unroll
+      for (uint32_t half = 8; half > 0; half /= 2) {
+        const uint32_t n = wave_sum(up_to(lo + half));
+        if (n <= id) lo += half, below = n;
+      }
+      const uint32_t before = up_to(lo), mine = up_to(lo + 1) - before;
+      const uint32_t end = wave_scan(mine);
+      past = __ballot(end > id - below);
+      local = before + (id - below) - (end - mine);
+    }
+  }
   if (past == 0) return it;
   const int owner = __builtin_ctzll(past);
-  // In the owner lane: which of its requests, and the index within it.
-  uint32_t local = id - (unit_end - units), first = item_end - items;
+  uint32_t first = item_end - items;
   uint32_t e_found = 0, n_splits = splits[0], n_tiles = tiles[0], n_blocks = blocks[0],
            n_whole = whole[0];
   Request y = x[0];
@@ -324,7 +381,9 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, uint32_t id) {
   it.split = one || TILES ? 0 : rest - (t - n_whole) * n_splits;
   // The last tile first: with a causal mask it sees the most keys.
   it.tile = n_tiles - 1 - t;
-  it.index = (TILES ? first + n_whole + rest * n_splits : id) - full;
+  it.index = first + (TILES ? n_whole + rest * n_splits : local) - full;
+  // (More items than were launched: requests that overlap.)
+  if (!one && static_cast<uint32_t>(it.index) >= a.items) it.r = -1;
   return it;
 }
 
@@ -1300,16 +1359,15 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   if (requests > 0 && requests <= kPlanRequests && blocks > kMinChunk && p.tiles < 8 * round &&
       kv_heads <= slots && !full) {
     // A split tile's last range is half full on average: split_target + tiles / 2
-    // items come of it, and are meant to fill rounds: one where tiles are few (a
-    // little under it: unequal requests have more tiles; 32 requests of 16 tokens
-    // 52.9 us, with round - tiles 57.3, round - tiles / 2 51.2, but 10 of chunks and
-    // single tokens 108.7, 108.3, 110.2), else two or, of single tokens, up to three
-    // (24 single tokens 83.2 us with 1.5 rounds, 94 with one, 87 with two; 64 of them
-    // 148 with two rounds, 160 with 1.5, 168 with one).
-    if (2 * alike <= round)
-      p.split_target = round - 3 * alike / 4;
-    else
-      p.split_target = !p.few ? round : alike <= round ? 3 * round / 2 : 2 * round;
+    // items come of it. Where tiles are few they are meant to fill one round, or a
+    // little less, unequal requests having more tiles (32 requests of 16 tokens 52.9
+    // us; with round - tiles 57.3, round - tiles / 2 51.2; 10 of chunks and single
+    // tokens 108.7, 108.3, 110.2). Else (single tokens of 48 and 64 requests 112 and
+    // 141 us; with one round 113 and 142, with two 117 and 143; of 128 requests 208,
+    // 220, 211; chunks beside single tokens: 95.5 us with one round, 98.7 with 0.75,
+    // 95.3 with 1.5, 102 with two).
+    if (2 * alike <= round) p.split_target = round - 3 * alike / 4;
+    else p.split_target = p.few ? 3 * round / 2 : round;
   }
   const int64_t most = p.tiles * (blocks / kMinChunk + 1);
   p.items = p.tiles + p.split_target < most ? p.tiles + p.split_target : most;

@@ -682,3 +682,65 @@ def test_forward_only(dev):
     with pytest.warns(UserWarning, match="autograd kernel was not registered"):
         out.sum().backward()
     assert q.grad is None
+
+
+@pytest.mark.parametrize("causal", (True, False))
+@pytest.mark.parametrize("R,top,cached", ((2, 700, 0), (9, 300, 900), (40, 1, 1500), (64, 1, 300),
+                                          (64, 40, 500), (30, 200, 20)))
+@pytest.mark.parametrize("D", (64, 256))
+def test_longest_items_first(dev, D, R, top, cached, causal):
+    """More items than the GPU runs at once, of up to 64 requests of all lengths, nothing among
+    them: every row is written, by the item it belongs to."""
+    H, heads = 64, [0, 40]
+    g = torch.Generator().manual_seed(R + top)
+    new = torch.randint(0 if R > 2 else 1, top + 1, (R,), generator=g).tolist()
+    ctx = (torch.rand(R, generator=g) ** 3 * cached).int().tolist()
+    if cached:
+        ctx[R // 2] = cached
+    if top == 1:
+        new = [1] * R
+    new[0] = top
+    P, keys = 16, [n + c for n, c in zip(new, ctx)]
+    need = [-(-m // P) for m in keys]
+    table, at = torch.full((R, max(need)), -1, dtype=torch.int32), 0
+    for r, n in enumerate(need):
+        table[r, :n] = torch.arange(at, at + n)
+        at += n
+    q = randn((sum(new), H, D), BF16, R, 1.3)
+    pk, pv = randn((at, P, H, D), BF16, R + 1, 1.3), randn((at, P, H, D), BF16, R + 2)
+    cu = cu_of(new)
+    out = torch.full(q.shape, math.nan, dtype=BF16, device=dev)
+    jo.attention_paged(q.to(dev), pk.to(dev), pv.to(dev), table.to(dev), i32(cu, dev), i32(keys, dev),
+                       causal=causal, out=out)
+    reqs = []
+    for r in range(R):
+        k, v = (x[table[r, :need[r]].long()].flatten(0, 1)[:keys[r], heads] for x in (pk, pv))
+        reqs.append((cu[r], cu[r + 1], k, v, seen_mask(new[r], keys[r], causal)))
+    assert bool(torch.isfinite(out).all())
+    check(out[:, heads], q[:, heads], reqs, D ** -0.5, BF16)
+    if cached == 0:
+        cut = randn((sum(new), H, D), BF16, 5), randn((sum(new), H, D), BF16, 6)
+        out.fill_(math.nan)
+        jo.attention_varlen(q.to(dev), cut[0].to(dev), cut[1].to(dev), i32(cu, dev), causal=causal, out=out)
+        reqs = [(cu[r], cu[r + 1], cut[0][cu[r]:cu[r + 1], heads], cut[1][cu[r]:cu[r + 1], heads],
+                 seen_mask(new[r], new[r], causal)) for r in range(R)]
+        assert bool(torch.isfinite(out).all())
+        check(out[:, heads], q[:, heads], reqs, D ** -0.5, BF16)
+
+
+def test_sequences_that_overlap_stay_inside(dev):
+    """cu_q that is not sorted gives more rows than tokens: no result is promised for them, but
+    nothing outside the call's tensors changes."""
+    T, H, D, P = 200, 16, 128, 16
+    q = randn((T, H, D), BF16, 1).to(dev)
+    pk = randn((64, P, H, D), BF16, 2).to(dev)
+    table = torch.arange(64, dtype=torch.int32, device=dev).view(8, 8)
+    big = torch.full((T + 64, H, D), 5.0, dtype=BF16, device=dev)
+    for cu in ([0, 200, 0, 200, 0, 200, 0, 200, 0], [0, -5, 300, 10, 2 ** 31 - 1, 7, 200, 3, 200],
+               [200, 0, 0, 0, 0, 0, 0, 0, 200]):
+        for causal in (True, False):
+            jo.attention_paged(q, pk, pk, table, i32(cu, dev), i32([128] * 8, dev), causal=causal,
+                               out=big[32:T + 32])
+            jo.attention_varlen(q, q, q, i32(cu, dev), causal=causal, out=big[32:T + 32])
+            torch.cuda.synchronize(dev)
+            assert bool((big[:32] == 5).all()) and bool((big[T + 32:] == 5).all())
