@@ -1002,12 +1002,11 @@ __global__ __launch_bounds__(kBlock, D <= 128 ? 2 : 1) void attn_tiles_kernel(co
 // no other wave until the waves' results are joined at the end.
 //
 // Bound by reading the keys once: 64 requests of 100 to 16384 keys, 8 key heads
-// of 128, 148 us (5.0 TB/s; a large copy moves 5.15), two of 100000 keys 95 us
+// of 128, 141 us (5.2 TB/s; a large copy moves 5.15), two of 100000 keys 95 us
 // (5.3), 256 of 500 to 2000 211 us (5.3); four of 300 to 2000 keys 11 us, of
-// which the joining kernel takes 3 and a launch 4: latency. Measured level: four
-// or two waves a workgroup (the latter 4 to 8% slower in full batches), page ids
-// of 32 blocks at a time. Items that share an XCD by request instead of by key
-// head: 64 requests 148 -> 203 us.
+// which the joining kernel takes 3 and a launch 4: latency. Two waves a workgroup
+// were 4 to 8% slower in full batches, page ids of 32 blocks at a time level; items
+// that share an XCD by request instead of by key head: 64 requests 148 -> 203 us.
 // ---------------------------------------------------------------------------
 template <int D>
 struct FewShape {
