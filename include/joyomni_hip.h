@@ -544,7 +544,8 @@ int jo_paged_tables(const int32_t* ctx_lens, const int32_t* new_lens, int64_t re
  * out. Slots of one call must differ (of two rows sent to one place parts of
  * either may remain). src: [layers, tokens, num_heads * head_dim]; pages:
  * [layers, num_pages, page_size, num_heads * head_dim], element strides, token
- * rows contiguous; fewer than 2^32 tokens in a pool. */
+ * rows contiguous, in any order that keeps rows apart; fewer than 2^32 tokens in
+ * a pool. */
 int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, void* pages_k, void* pages_v,
                             int64_t layers, int64_t tokens, int64_t num_heads, int64_t head_dim,
                             int64_t src_layer_stride, int64_t src_token_stride,

@@ -26,6 +26,7 @@
 // contiguous form: 1560 tokens of 32 x 128, 40 layers, K and V, 334 us (6.1 TB/s
 // of rows read and written); 32 single tokens of one layer 3.2 us, a launch.
 
+#include <algorithm>
 #include <type_traits>
 
 #include "jo_device.hpp"
@@ -226,8 +227,8 @@ int launch_commit(const CommitArgs& args, hipStream_t stream) {
                       al(a.src_v, a.s_ls) && al(a.src_v, a.s_bs) && al(a.src_v, a.s_ts) &&
                       al(a.dst_k, a.d_ls) && al(a.dst_k, a.d_bs) && al(a.dst_k, a.d_ts) &&
                       al(a.dst_v, a.d_ls) && al(a.dst_v, a.d_bs) && al(a.dst_v, a.d_ts) &&
-                      al(a.dst_k, a.d_ps) && al(a.dst_v, a.d_ps) && aligned(a.cos, 16) && aligned(a.sin, 16) && a.tab_ts % 4 == 0 &&
-                      a.tab_bs % 4 == 0;
+                      al(a.dst_k, a.d_ps) && al(a.dst_v, a.d_ps) && aligned(a.cos, 16) &&
+                      aligned(a.sin, 16) && a.tab_ts % 4 == 0 && a.tab_bs % 4 == 0;
   const int chunks = (a.row_elems + 511) / 512;
   // K and V on separate waves: 40 x 1560 x [32, 128] 357 -> 340 us (twice the
   // waves, each streaming one tensor). The JO_KNOB_KV_SPLIT override 1 keeps
@@ -238,9 +239,11 @@ int launch_commit(const CommitArgs& args, hipStream_t stream) {
   auto go = [&](auto ch) {
     constexpr int CH = decltype(ch)::value;
     if (kv2)
-      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, true, PAGED, ROPE>), grid, dim3(kBlock), 0, stream, a);
+      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, true, PAGED, ROPE>), grid, dim3(kBlock), 0,
+                         stream, a);
     else
-      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, false, PAGED, ROPE>), grid, dim3(kBlock), 0, stream, a);
+      hipLaunchKernelGGL((rope_commit_kernel<Tag, CH, false, PAGED, ROPE>), grid, dim3(kBlock), 0,
+                         stream, a);
   };
   if (vec_ok && chunks <= 1)
     go(std::integral_constant<int, 1>{});
@@ -340,6 +343,19 @@ extern "C" int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, voi
   JO_REQUIRE(rows <= int64_t{UINT32_MAX} / (2 * 64), "%s: too many rows (%lld, at most %lld)", op,
              static_cast<long long>(rows), static_cast<long long>(int64_t{UINT32_MAX} / (2 * 64)));
   JO_REQUIRE(src_k && pages_k && slots, "%s: null pointer", op);
+  // Layers, pages and places, from the smallest stride on: each steps over all
+  // that those before it reach, or two rows of the pool would share elements.
+  struct Dim {
+    int64_t n, stride;
+  } dims[] = {{layers, pages_layer_stride}, {num_pages, page_stride}, {page_size, pages_token_stride}};
+  std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  int64_t reach = num_heads * head_dim;
+  for (const Dim& d : dims) {
+    if (d.n <= 1) continue;
+    JO_REQUIRE(d.stride >= reach, "%s: rows of the pages must not overlap (bad stride)", op);
+    JO_REQUIRE(d.stride <= (INT64_MAX / 2 - reach) / (d.n - 1), "%s: pool too large", op);
+    reach += (d.n - 1) * d.stride;
+  }
   CommitArgs a{src_k, src_v, pages_k, pages_v, layers, 1, tokens,
                static_cast<int>(num_heads * head_dim), static_cast<int>(head_dim),
                src_layer_stride, 0, src_token_stride, pages_layer_stride, 0, pages_token_stride, 0,

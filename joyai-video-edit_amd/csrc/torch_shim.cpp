@@ -1243,7 +1243,8 @@ void attn_no_overlap(const torch::Tensor& out, std::initializer_list<const torch
 
 void attn_workspace(AttnCall& c, const torch::Tensor& q, int64_t kv_capacity, bool causal) {
   c.ws_bytes = jo_attention_workspace_bytes(c.T, c.R, c.Hq, c.Hkv, c.D, kv_capacity, causal);
-  if (c.ws_bytes > 0) c.ws = torch::empty({c.ws_bytes}, q.options().dtype(torch::kUInt8));
+  if (c.ws_bytes > 0)
+    c.ws = at::detail::empty_cuda({c.ws_bytes}, q.options().dtype(torch::kUInt8));
 }
 
 void run_varlen(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
@@ -1297,7 +1298,7 @@ torch::Tensor attn_out(const torch::Tensor& q) {
   JO_CHECK_CUDA(q);
   TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(q.device());
-  return torch::empty(q.sizes(), q.options());
+  return at::detail::empty_cuda(q.sizes(), q.options());
 }
 }  // namespace
 

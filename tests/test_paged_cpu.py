@@ -79,6 +79,9 @@ REFUSED += [
     (paged(ot=392, oh=128), "overlap"), (varlen(ot=128, oh=504), "overlap"),
     # Rows of K and V that 32 bits do not reach.
     (varlen(kt=2 ** 24), "stride"), (paged(vp=2 ** 36, N=8), "64 GiB"),
+    # Rows of the pool that share elements: pages, layers, places.
+    (commit(pp=0), "overlap"), (commit(pp=3900), "overlap"), (commit(L=3, pl=4096), "overlap"),
+    (commit(L=3, pl=0), "overlap"), (commit(pp=256, pt=256), "overlap"), (commit(pp=2 ** 62), "too large"),
     # Results in the place of what other workgroups still read.
     (tables(kv=P, cu=P + 2 ** 16, slots=P + 2 ** 17, table=P + 2 ** 18), "overlaps an input"),
     (tables(kv=P + 2 ** 15, cu=P + 2 ** 16, slots=P + 2 ** 17, table=P + 8), "overlaps an input"),
