@@ -478,14 +478,21 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 #define JO_LDS(type, addr) \
   ((__attribute__((address_space(3))) type*)(static_cast<uintptr_t>(addr)))
 
+__device__ __forceinline__ uint32_t lds_address(char* shared) {
+  return static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)shared));
+}
+
 __device__ __forceinline__ u32x4 lds_read16(uint32_t addr) { return *JO_LDS(u32x4, addr); }
 
 // Two transposing reads: within each 16 lanes, lane i names four consecutive
 // elements of row i / 4 and gets column i of the 4 x 16 block: four rows of its
 // own column. Rows here are keys, columns places of head_dim.
 __device__ __forceinline__ u32x4 lds_read_tr(uint32_t addr0, uint32_t addr1) {
-  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr0)));
-  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr1)));
+  const u32x2 a =
+      __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr0)));
+  const u32x2 b =
+      __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(JO_LDS(i16x4, addr1)));
   return u32x4{a.x, a.y, b.x, b.y};
 }
 
@@ -496,7 +503,6 @@ __device__ __forceinline__ u32x4 lds_read_tr(uint32_t addr0, uint32_t addr1) {
 // Keeps memory accesses on their side of it (the compiler does not know what the
 // waits above wait for).
 #define JO_KEEP_ORDER() asm volatile("" ::: "memory")
-
 
 // A key row of D elements is D / 8 chunks of 16 bytes; chunk c of row r of a
 // tile in LDS sits at chunk position c ^ swz(r). The 32 banks of 8 bytes hold
@@ -556,7 +562,8 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Request& x,
 // the two LDS buffers apart, would wait for the block being loaded before the
 // transposing reads of the other one; the waits are where the blocks are used.
 // (Of its own loads it then knows too few to be behind them, and waits longer
-// than it must, never shorter.)
+// than it must, never shorter.) m0, which no compiled code here uses otherwise,
+// is set by every load for itself.
 __device__ __forceinline__ void load_to_lds(const char* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                :
@@ -615,7 +622,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const Item& it, int
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) store_elem<Tag>(a.out, off + e * 64 + lane, o[e] * inv);
   } else {
-    float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * rows_per_tile * (D + 2);
+    float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * rows_per_tile *
+                             (D + 2);
 #pragma unroll
     for (int e = 0; e < D / 64; ++e) part[local_row * D + e * 64 + lane] = o[e];
     if (lane == 0) {
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(kBlock, D <= 128 ? 2 : 1) void attn_tiles_kernel(co
   constexpr int COUNT = kKeyBlock / PER / WAVES;
   constexpr int KK = D / 16, DB = D / 32;
   __shared__ __attribute__((aligned(1024))) char smem[4 * BLOCK];  // K0 K1 V0 V1
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const uint32_t lds = lds_address(smem);
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t id = blockIdx.x;
@@ -1025,7 +1033,7 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
   constexpr int KK = D / 32, DB = D / 16;
   __shared__ __attribute__((aligned(1024))) char smem[W * S::kWaveBytes];
   __shared__ float s_m[W][ROWS], s_l[W][ROWS];
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const uint32_t lds = lds_address(smem);
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t id = blockIdx.x;
@@ -1081,53 +1089,53 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
   constexpr int STEP = W * S::kKeys;  // a wave's blocks are this far apart
   const int my_begin = k_begin + wave * S::kKeys;
   auto attend = [&](int base, int buf, uint32_t there) JO_INLINE {
-          f32x4 s[2] = {};
-          const uint32_t ka = k_addr + buf * BLOCK;
-    #pragma unroll
-          for (int k = 0; k < KK; ++k)
-    #pragma unroll
-            for (int b = 0; b < 2; ++b)
-              s[b] = mfma16<Tag>(lds_read16((ka ^ (k << 6)) + b * 16 * D * 2), q[k], s[b]);
-          if (base + S::kKeys > first_end || ~there != 0) {
-    #pragma unroll
-            for (int b = 0; b < 2; ++b)
-    #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int j = b * 16 + grp * 4 + e;
-                if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
-              }
-          }
-          float top = fmaxf(s[0][0], s[1][0]);
-    #pragma unroll
-          for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
-          if (__any(top * a.scale_log2 > m + kLazyMax)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m, top * a.scale_log2);
-            const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
-            m = m_new;
-            l *= fade;
-    #pragma unroll
-            for (int d = 0; d < DB; ++d)
-    #pragma unroll
-              for (int e = 0; e < 4; ++e) o[d][e] *= fade;
-          }
-          const float m_use = m == -INFINITY ? 0.f : m;
-          float w[8];
-    #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            w[e] = exp2_fast(fmaf(s[e / 4][e % 4], a.scale_log2, -m_use));
-            l += w[e];
-          }
-          const u32x4 p = {pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
-                           pack2<Tag>(w[6], w[7])};
-          const uint32_t va = v_addr + buf * BLOCK;
-          const int sw0 = swz_k<D>(v_row), sw1 = swz_k<D>(v_row + 16);
-    #pragma unroll
-          for (int d = 0; d < DB; ++d)
-            o[d] = mfma16<Tag>(lds_read_tr(va + (((d * 2 + v_chunk) ^ sw0) << 4),
-                                           va + 16 * D * 2 + (((d * 2 + v_chunk) ^ sw1) << 4)),
-                               p, o[d]);
+    f32x4 s[2] = {};
+    const uint32_t ka = k_addr + buf * BLOCK;
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = mfma16<Tag>(lds_read16((ka ^ (k << 6)) + b * 16 * D * 2), q[k], s[b]);
+    if (base + S::kKeys > first_end || ~there != 0) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = b * 16 + grp * 4 + e;
+          if (base + j >= my_end || !((there >> j) & 1)) s[b][e] = -INFINITY;
+        }
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[0][e], s[1][e]));
+    if (__any(top * a.scale_log2 > m + kLazyMax)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m_new = fmaxf(m, top * a.scale_log2);
+      const float fade = m_new == -INFINITY ? 1.f : exp2_fast(m - m_new);
+      m = m_new;
+      l *= fade;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= fade;
+    }
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = exp2_fast(fmaf(s[e / 4][e % 4], a.scale_log2, -m_use));
+      l += w[e];
+    }
+    const u32x4 p = {pack2<Tag>(w[0], w[1]), pack2<Tag>(w[2], w[3]), pack2<Tag>(w[4], w[5]),
+                     pack2<Tag>(w[6], w[7])};
+    const uint32_t va = v_addr + buf * BLOCK;
+    const int sw0 = swz_k<D>(v_row), sw1 = swz_k<D>(v_row + 16);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      o[d] = mfma16<Tag>(lds_read_tr(va + (((d * 2 + v_chunk) ^ sw0) << 4),
+                                     va + 16 * D * 2 + (((d * 2 + v_chunk) ^ sw1) << 4)),
+                         p, o[d]);
   };
   if (my_begin < k_end) {
     // Page ids run two blocks ahead of the loads that they are for: in order with
@@ -1186,7 +1194,8 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
     const float mw = s_m[w][row];
     const float e = mw == -INFINITY ? (mw == top ? 1.f : 0.f) : exp2_fast(mw - top);
     sum = fmaf(e, s_l[w][row], sum);
-    const float* src = reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + row * S::kRowFloats;
+    const float* src =
+        reinterpret_cast<const float*>(smem + w * S::kWaveBytes) + row * S::kRowFloats;
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(src + (n * TPR + part_of) * 4);
@@ -1210,7 +1219,8 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
 #pragma unroll
       for (int n = 0; n < NE; ++n)
         st8(out + (n * TPR + part_of) * 4 * Tag::kBytes,
-            u32x2{pack2<Tag>(r[n][0] * inv, r[n][1] * inv), pack2<Tag>(r[n][2] * inv, r[n][3] * inv)});
+            u32x2{pack2<Tag>(r[n][0] * inv, r[n][1] * inv),
+                  pack2<Tag>(r[n][2] * inv, r[n][3] * inv)});
     } else {
       float* part = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
 #pragma unroll
@@ -1228,8 +1238,8 @@ __global__ __launch_bounds__(FewShape<D>::kWaves* kWave, 1) void attn_few_kernel
     const int local = wave * (kWave / TPR) + b;
     const int i = fdiv(row0 + local, a.fd_group);
     float ro[D / 64], rm, rl;
-    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row0 + local - i * a.group, i, k_begin,
-                              min(k_end, visible(a, x, i)), rm, rl, ro);
+    attend_row<Tag, D, PAGED>(a, it.r, x, kv_head * a.group + row0 + local - i * a.group, i,
+                              k_begin, min(k_end, visible(a, x, i)), rm, rl, ro);
     store_row<Tag, D>(a, it, kv_head, row0 + local, local, ROWS, rm, rl, ro);
   }
 }
@@ -1255,7 +1265,8 @@ __global__ __launch_bounds__(kBlock) void attn_join_kernel(const AttnArgs a) {
   if (it.r < 0 || it.splits == 1 || static_cast<uint32_t>(it.index + it.splits) > a.items) return;
   const int rows = min(ROWS, it.x.nq * a.group - it.tile * ROWS);
   const int64_t stride = static_cast<int64_t>(a.kv_heads) * ROWS * (D + 2);
-  const float* first = a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
+  const float* first =
+      a.ws + (static_cast<int64_t>(it.index) * a.kv_heads + kv_head) * ROWS * (D + 2);
   const int c = threadIdx.x % C, group = threadIdx.x / C % GROUPS;
 #pragma unroll 1
   for (int row0 = row_begin; row0 < min(rows, row_begin + PER * EACH); row0 += PER) {
@@ -1335,12 +1346,13 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t requests, int64_t q_heads, int
   const int64_t all_rows = q_tokens * group;
   p.few = all_rows <= 16 * requests;
   const int64_t rows = p.few ? 16 : kTileRows;
-  p.tiles = all_rows / rows + (requests < q_tokens || requests > kPlanRequests ? requests : q_tokens);
+  p.tiles =
+      all_rows / rows + (requests < q_tokens || requests > kPlanRequests ? requests : q_tokens);
   if (requests == 0) p.tiles = 0;
   const int64_t blocks = (kv_capacity + kKeyBlock - 1) / kKeyBlock;
   // Workgroups that run at once: LDS and registers let two of the smaller ones
   // share a compute unit.
-  const int64_t slots = kComputeUnits * (p.few ? (head_dim == 64 ? 2 : 1) : (head_dim <= 128 ? 2 : 1));
+  const int64_t slots = kComputeUnits * (head_dim <= (p.few ? 64 : 128) ? 2 : 1);
   const int64_t round = (slots + kv_heads - 1) / kv_heads;  // items of one round
   p.split_target = 0;
   // How many tiles there are if the requests are alike.
@@ -1405,7 +1417,8 @@ template <class Tag, int D, bool PAGED>
 int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes,
                      hipStream_t stream) {
   const char* op = PAGED ? "attention_paged" : "attention_varlen";
-  AttnPlan p = plan_attention(a.q_tokens, a.requests, a.q_heads, a.kv_heads, D, kv_capacity, a.causal);
+  AttnPlan p =
+      plan_attention(a.q_tokens, a.requests, a.q_heads, a.kv_heads, D, kv_capacity, a.causal);
   if (p.ws_bytes > 0 && ws_bytes < p.ws_bytes) {  // none, or one for another call: no splits
     p.split_target = 0;
     p.tail_splits = 1;
@@ -1429,9 +1442,11 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
     hipLaunchKernelGGL((attn_few_kernel<Tag, D, PAGED>), grid, dim3(FewShape<D>::kWaves * kWave), 0,
                        stream, a);
   else if constexpr (!PAGED)
-    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPacked>), grid, dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPacked>), grid, dim3(kBlock), 0, stream,
+                       a);
   else if (a.fd_page.d % 16 == 0)
-    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages16>), grid, dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages16>), grid, dim3(kBlock), 0, stream,
+                       a);
   else
     hipLaunchKernelGGL((attn_tiles_kernel<Tag, D, Keys::kPages>), grid, dim3(kBlock), 0, stream, a);
   int st = launch_status(op);
@@ -1446,11 +1461,11 @@ int launch_attention(AttnArgs a, int64_t kv_capacity, void* ws, int64_t ws_bytes
   JO_REQUIRE(joins <= INT32_MAX / 512, "%s: shape too large", op);
   const dim3 join(static_cast<unsigned>(joins));
   if (p.few)
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED, kFewJoin, 1>), join, dim3(kBlock), 0, stream,
-                       a);
-  else
-    hipLaunchKernelGGL((attn_join_kernel<Tag, D, kTileRows, PAGED, kTileJoin, kTileEach>), join, dim3(kBlock), 0,
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, 16, PAGED, kFewJoin, 1>), join, dim3(kBlock), 0,
                        stream, a);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<Tag, D, kTileRows, PAGED, kTileJoin, kTileEach>), join,
+                       dim3(kBlock), 0, stream, a);
   return launch_status(op);
 }
 
@@ -1565,9 +1580,11 @@ extern "C" int jo_attention_varlen(const void* q, const void* k, const void* v, 
   a.causal = causal != 0;
   a.fill_rest = fill_rest != 0;
   if (const int bad = key_offsets(op, a, 1, kv_tokens); bad != JO_OK) return bad;
-  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16), "%s: workspace must be 16-byte aligned", op);
+  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16),
+             "%s: workspace must be 16-byte aligned", op);
   return dispatch_attention<false>(a, head_dim, dtype, kv_tokens, workspace,
-                                   workspace ? workspace_bytes : 0, static_cast<hipStream_t>(stream));
+                                   workspace ? workspace_bytes : 0,
+                                   static_cast<hipStream_t>(stream));
 }
 
 extern "C" int jo_attention_paged(const void* q, const void* pages_k, const void* pages_v,
@@ -1609,9 +1626,11 @@ extern "C" int jo_attention_paged(const void* q, const void* pages_k, const void
   a.causal = causal != 0;
   a.fill_rest = fill_rest != 0;
   if (const int bad = key_offsets(op, a, num_pages, page_size); bad != JO_OK) return bad;
-  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16), "%s: workspace must be 16-byte aligned", op);
+  JO_REQUIRE(workspace_bytes >= 0 && aligned(workspace, 16),
+             "%s: workspace must be 16-byte aligned", op);
   return dispatch_attention<true>(a, head_dim, dtype, table_width * page_size, workspace,
-                                  workspace ? workspace_bytes : 0, static_cast<hipStream_t>(stream));
+                                  workspace ? workspace_bytes : 0,
+                                  static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t jo_attention_workspace_bytes(int64_t q_tokens, int64_t requests,

@@ -347,7 +347,9 @@ extern "C" int jo_kv_commit_rope_paged(const void* src_k, const void* src_v, voi
   // that those before it reach, or two rows of the pool would share elements.
   struct Dim {
     int64_t n, stride;
-  } dims[] = {{layers, pages_layer_stride}, {num_pages, page_stride}, {page_size, pages_token_stride}};
+  } dims[] = {{layers, pages_layer_stride},
+              {num_pages, page_stride},
+              {page_size, pages_token_stride}};
   std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
   int64_t reach = num_heads * head_dim;
   for (const Dim& d : dims) {
